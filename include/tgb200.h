@@ -319,6 +319,32 @@ int tg_cross_entropy_backward(int dtype, const void* logits, const int64_t* targ
                               void* grad, int64_t rows, int64_t classes, int64_t ignore_index,
                               int reduction, void* stream);
 
+/* ------------------------------------------------------------------ scores of tokens
+ * Under logits (rows, classes), class axis last (no reference counterpart): per row, with m =
+ * max x and s = sum exp(x - m) written to stats[row] = (m, s) for the VJP,
+ *   log_probs[row] = x[t] - m - log s  (0 where t == ignore_index; a target outside [0, classes)
+ *                    that is not ignore_index sets *bad_target_dev, int32, and gives 0),
+ *   entropy[row]   = -sum p log p,
+ *   top_log_probs[row][k], top_ids[row][k]: the top_k largest entries' log probabilities and
+ *                    classes in descending order, equal entries by ascending class, NaN last.
+ * Entries of -inf have probability 0 and add nothing. A row of -inf alone, or with a NaN or
+ * +inf, gives NaN (its top_ids stay distinct classes). top_k <= tg_token_log_probs_max_top().
+ * `scratch`: tg_token_log_probs_scratch_bytes(dtype, rows, classes, top_k). */
+int tg_token_log_probs_max_top(void);
+size_t tg_token_log_probs_scratch_bytes(int dtype, int64_t rows, int64_t classes, int64_t top_k);
+int tg_token_log_probs_forward(int dtype, const void* logits, const int64_t* targets, void* stats,
+                               void* log_probs, void* entropy, void* top_log_probs,
+                               int64_t* top_ids, int64_t rows, int64_t classes, int64_t top_k,
+                               int64_t ignore_index, int* bad_target_dev, void* scratch,
+                               void* stream);
+/* grad[row][j] = g_log[row] [j == t] + sum_k g_top[row][k] [j == top_ids[row][k]]
+ *   - p_j (g_log[row] + sum_k g_top[row][k] + g_ent[row] (log p_j + entropy[row])). */
+int tg_token_log_probs_backward(int dtype, const void* logits, const int64_t* targets,
+                                const void* stats, const void* entropy, const int64_t* top_ids,
+                                const void* g_log, const void* g_ent, const void* g_top,
+                                void* grad, int64_t rows, int64_t classes, int64_t top_k,
+                                int64_t ignore_index, void* stream);
+
 /* ------------------------------------------------------------------ attention
  * Fused causal/non-causal softmax attention (ops/attention.py:71-116, 163-272) as a flash-
  * style kernel: the forward stores O and the row log-sum-exp instead of P; the backward

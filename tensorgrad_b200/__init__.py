@@ -14,7 +14,8 @@ from tensorgrad_b200.ops import (
     add, binary_cross_entropy_with_logits, broadcast_to, concat, conv2d, cross_entropy, div,
     dropout, embedding, exp, flatten, gelu, layer_norm, linear, log, log_softmax, logsumexp,
     masked_fill, matmul, max, max_pool2d, mean, min, mse_loss, mul, neg, permute, pow, relu,
-    reshape, sigmoid, softmax, sqrt, squeeze, stack, sub, sum, tanh, transpose, unsqueeze, var,
+    reshape, sigmoid, softmax, sqrt, squeeze, stack, sub, sum, tanh,
+    token_log_probs, transpose, unsqueeze, var,
     where,
 )
 from tensorgrad_b200.tensor import (
@@ -42,6 +43,6 @@ __all__ = [
     "mean", "min", "mse_loss", "mul", "neg", "nn", "no_grad", "ones", "ones_like", "optim",
     "permute", "pow", "profiler", "rand", "randn", "relu", "reshape", "set_default_dtype",
     "set_device", "sigmoid", "softmax", "sqrt", "squeeze", "stack", "sub", "sum", "synchronize",
-    "tanh", "tensor", "transpose", "unsqueeze", "utils", "var", "viz", "where", "zeros",
+    "tanh", "tensor", "token_log_probs", "transpose", "unsqueeze", "utils", "var", "viz", "where", "zeros",
     "zeros_like",
 ]

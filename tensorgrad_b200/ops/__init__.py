@@ -9,7 +9,9 @@ from tensorgrad_b200.ops.elementwise import (
 )
 from tensorgrad_b200.ops.layers import batch_norm, dropout, embedding, layer_norm, linear
 from tensorgrad_b200.ops.linalg import matmul
-from tensorgrad_b200.ops.loss import binary_cross_entropy_with_logits, cross_entropy, mse_loss
+from tensorgrad_b200.ops.loss import (
+    TokenLogProbs, binary_cross_entropy_with_logits, cross_entropy, mse_loss, token_log_probs,
+)
 from tensorgrad_b200.ops.recurrent import gru, lstm, rnn
 from tensorgrad_b200.ops.reduce import max, mean, min, sum, var
 from tensorgrad_b200.ops.shape import (
@@ -18,11 +20,11 @@ from tensorgrad_b200.ops.shape import (
 )
 
 __all__ = [
-    "add", "astype", "batch_norm", "binary_cross_entropy_with_logits", "broadcast_to", "concat",
+    "TokenLogProbs", "add", "astype", "batch_norm", "binary_cross_entropy_with_logits", "broadcast_to", "concat",
     "conv2d", "cross_entropy", "div", "dropout", "embedding", "exp", "flatten", "gelu", "getitem",
     "gru", "layer_norm", "linear", "log", "log_softmax", "logsumexp", "lstm", "masked_fill",
     "matmul", "max", "max_pool2d", "mean", "min", "mse_loss", "mul", "neg",
     "packed_self_attention", "permute", "pow", "relu", "reshape", "rnn",
     "scaled_dot_product_attention", "sigmoid", "softmax", "sqrt", "squeeze", "stack", "sub",
-    "sum", "sum_to", "tanh", "transpose", "unsqueeze", "var", "where",
+    "sum", "sum_to", "tanh", "token_log_probs", "transpose", "unsqueeze", "var", "where",
 ]

@@ -1,8 +1,9 @@
-"""Loss functions (the reference's ops/loss.py)."""
+"""Loss functions (the reference's ops/loss.py) and the scores of tokens under logits."""
 
 from __future__ import annotations
 
-from typing import Any, Literal
+import math
+from typing import Any, Literal, NamedTuple
 
 import numpy as np
 
@@ -10,12 +11,15 @@ from tensorgrad_b200 import device
 from tensorgrad_b200._lib import check, lib
 from tensorgrad_b200.device import DeviceArray, dtype_code
 from tensorgrad_b200.ops import reduce
-from tensorgrad_b200.ops._util import Need, as_tensor, coerce_pair, make_result
+from tensorgrad_b200.ops._util import (
+    Need, as_tensor, coerce_pair, graph_by_composite, make_result,
+)
 from tensorgrad_b200.ops.elementwise import cast_array
 from tensorgrad_b200.profiler import profiled
 from tensorgrad_b200.tensor import Tensor
 
-__all__ = ["Reduction", "binary_cross_entropy_with_logits", "cross_entropy", "mse_loss"]
+__all__ = ["Reduction", "TokenLogProbs", "binary_cross_entropy_with_logits", "cross_entropy",
+           "mse_loss", "token_log_probs"]
 
 Reduction = Literal["mean", "sum", "none"]
 _RED = {"mean": 0, "sum": 1, "none": 2}
@@ -181,3 +185,135 @@ def binary_cross_entropy_with_logits(logits: Any, target: Any, *,
                 -tz * up if need[1] else None)
 
     return make_result(out, (tz, ty), backward, "binary_cross_entropy", graph)
+
+
+class TokenLogProbs(NamedTuple):
+    """What :func:`token_log_probs` gives: per row the target's log probability and the
+    entropy, and per row and alternative its log probability and its class (``None`` without
+    alternatives)."""
+
+    log_probs: Tensor
+    entropy: Tensor
+    top_log_probs: Tensor | None
+    top_ids: Tensor | None
+
+
+def _class_targets(what: str, tl: Tensor, target: Any,
+                   ignore_index: int) -> tuple[DeviceArray, int | None]:
+    """Class targets of ``tl``'s rows on the device as int64, checked as
+    :func:`cross_entropy` checks them: host targets here, device-resident ones by the kernel
+    through the returned flag word."""
+    dev_t = target.data if isinstance(target, Tensor) else target
+    on_device = isinstance(dev_t, DeviceArray)
+    t = dev_t if on_device else np.asarray(target)
+    if t.dtype.kind not in "iu":
+        raise TypeError(f"{what} targets must be integers, got {t.dtype}")
+    if tl.shape[:-1] != t.shape:
+        raise ValueError(f"logits {tl.shape} and targets {t.shape} are incompatible")
+    if on_device:
+        tgt = t if t.dtype == np.int64 else cast_array(t, np.dtype(np.int64))
+        return tgt, device.async_error_word(device.ASYNC_CLASS_TARGET)
+    flat = np.ascontiguousarray(t.reshape(-1), dtype=np.int64)
+    if np.any((flat != ignore_index) & ((flat < 0) | (flat >= tl.shape[-1]))):
+        raise IndexError(f"target out of range for {tl.shape[-1]} classes")
+    return device.from_numpy(flat), None
+
+
+def _part(packed: Tensor, offset: int, shape: tuple[int, ...]) -> Tensor:
+    """A contiguous part of a packed result as a view; its VJP puts the gradient into zeros
+    of the packed size."""
+    total = packed.size
+    count = math.prod(shape)
+
+    def backward(g: DeviceArray, need: Need) -> tuple[DeviceArray]:
+        out = device.zeros((total,), g.dtype)
+        device.copy_into(out.flat_view(offset, count), g)
+        return (out,)
+
+    def graph(g: Tensor, y: Tensor, need: Need) -> tuple[Tensor]:
+        from tensorgrad_b200.ops.shape import _scatter, reshape
+
+        return (_scatter(reshape(g, (count,)), (total,), slice(offset, offset + count)),)
+
+    return make_result(packed.data.flat_view(offset, count, shape), (packed,), backward,
+                       "token_log_probs", graph)
+
+
+@profiled("token_log_probs")
+def token_log_probs(logits: Any, targets: Any, *, top_k: int = 0,
+                    ignore_index: int = -100) -> TokenLogProbs:
+    """The given tokens' log probabilities under ``softmax(logits)``, class axis last, with
+    the distribution's entropy and its ``top_k`` likeliest classes (in descending order, equal
+    ones by ascending class), all from one pass over the logits.
+
+    Rows whose target is ``ignore_index`` have log probability 0 (their entropy and
+    alternatives count). Logits of ``-inf`` close a class: probability 0, nothing added. A row
+    without a finite logit, or with a NaN or ``+inf``, gives NaN. Targets are checked as
+    :func:`cross_entropy` checks them. Log probabilities, entropy and the alternatives' log
+    probabilities are differentiable in the logits (``top_ids`` is a constant choice).
+    """
+    tl = as_tensor(logits)
+    if tl.ndim == 0 or tl.shape[-1] == 0:
+        raise ValueError(f"token_log_probs needs a class axis, got logits {tl.shape}")
+    lead, classes = tl.shape[:-1], tl.shape[-1]
+    most = min(int(lib.tg_token_log_probs_max_top()), classes)
+    if not 0 <= top_k <= most:
+        raise ValueError(f"top_k must be in [0, {most}] for {classes} classes, got {top_k}")
+    tgt, bad = _class_targets("token_log_probs", tl, targets, ignore_index)
+    x = tl.data if tl.dtype.kind == "f" else cast_array(tl.data, np.dtype(np.float64))
+    rows = math.prod(lead)
+    code = dtype_code(x.dtype)
+    es = x.itemsize
+    # One buffer: log probabilities, entropies, then (row, alternative) log probabilities.
+    packed = device.empty((rows * (2 + top_k),), x.dtype)
+    stats = device.empty((rows, 2), x.dtype)
+    ids = device.empty((*lead, top_k), np.int64) if top_k else None
+    scratch = device.scratch(lib.tg_token_log_probs_scratch_bytes(code, rows, classes, top_k))
+    check(lib.tg_token_log_probs_forward(
+        code, x.ptr, tgt.ptr, stats.ptr, packed.ptr, packed.ptr + rows * es,
+        packed.ptr + 2 * rows * es, ids.ptr if ids is not None else None, rows, classes, top_k,
+        ignore_index, bad, scratch.ptr, device.stream()), "token_log_probs")
+
+    def backward(g: DeviceArray, need: Need) -> tuple[DeviceArray]:
+        if g.dtype != x.dtype:
+            g = cast_array(g, x.dtype)
+        grad = device.empty(tl.shape, x.dtype)
+        check(lib.tg_token_log_probs_backward(
+            code, x.ptr, tgt.ptr, stats.ptr, packed.ptr + rows * es,
+            ids.ptr if ids is not None else None, g.ptr, g.ptr + rows * es, g.ptr + 2 * rows * es, grad.ptr, rows, classes, top_k,
+            ignore_index, device.stream()), "token_log_probs backward")
+        return (grad if grad.dtype == tl.dtype else cast_array(grad, tl.dtype),)
+
+    def graph(g: Tensor, y: Tensor, need: Need) -> tuple[Tensor | None, ...]:
+        return graph_by_composite((tl,), lambda t: _scores_composite(t, tgt, ids, rows, classes,
+                                                                     top_k, ignore_index),
+                                  g, need)
+
+    whole = make_result(packed, (tl,), backward, "token_log_probs", graph)
+    return TokenLogProbs(
+        _part(whole, 0, lead), _part(whole, rows, lead),
+        _part(whole, 2 * rows, (*lead, top_k)) if ids is not None else None,
+        Tensor._wrap(ids) if ids is not None else None)
+
+
+def _scores_composite(tl: Tensor, tgt: DeviceArray, ids: DeviceArray | None, rows: int,
+                      classes: int, top_k: int, ignore_index: int) -> Tensor:
+    """The packed result of :func:`token_log_probs` in differentiable ops, with the targets
+    and the alternatives found (read back to the host) as constants."""
+    from tensorgrad_b200.ops.activation import log_softmax
+    from tensorgrad_b200.ops.elementwise import exp, mul, neg
+    from tensorgrad_b200.ops.shape import concat, getitem, masked_fill, reshape
+
+    x = reshape(tl, (rows, classes))
+    lp = masked_fill(log_softmax(x, -1), np.isneginf(x.numpy()), 0.0)
+    # A closed class is left out of the entropy by p log p = 0.
+    p = masked_fill(exp(lp), np.isneginf(x.numpy()), 0.0)
+    t = tgt.numpy().reshape(-1)
+    kept = (t != ignore_index) & (t >= 0) & (t < classes)
+    at = np.arange(rows)
+    given = mul(getitem(lp, (at, np.where(kept, t, 0))), Tensor(kept.astype(lp.dtype)))
+    parts = [given, neg(reduce.sum(mul(p, lp), axis=-1))]
+    if ids is not None:
+        alt = ids.numpy().reshape(rows, top_k)
+        parts.append(reshape(getitem(lp, (at[:, None], alt)), (rows * top_k,)))
+    return concat(parts)
