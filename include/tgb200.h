@@ -394,6 +394,51 @@ int tg_attention_backward_dropout(int dtype, const tg_attn_shape* s, const void*
                                   uint32_t threshold, double keep_scale, void* scratch,
                                   void* stream);
 
+/* ------------------------------------------------------------------ paged key-value cache
+ * The cache of nn/attention.py:27-111 in pages, so that sequences of different lengths share
+ * one pool and prefixes (no reference counterpart). key_pages and value_pages each hold
+ * num_pages pages of (kv_heads, page_size, head_dim); position t of sequence b lies on page
+ * pages[b * max_pages + t / page_size] (int64, on the device), slot t % page_size. Entries of
+ * the table behind a sequence's last position are not read. A page id outside [0, num_pages),
+ * a negative length and a position off the table set *bad_page_dev (int32, may be NULL) to 1;
+ * writes there are left out, reads give unspecified values of the pool (attention) or zeros
+ * (gather). head_dim may be any size; multiples of 16 bytes on 16-byte boundaries move fastest.
+ *
+ * tg_paged_append writes tokens [0, tokens) of k and v (element strides for batch, head and
+ * position) to positions lengths[b] + [0, tokens) of each sequence. Two sequences that name
+ * the same page must not both write to it. */
+int tg_paged_append(int dtype, int64_t batch, int64_t tokens, int64_t kv_heads, int64_t head_dim,
+                    const void* k, int64_t k_sb, int64_t k_sh, int64_t k_st, const void* v,
+                    int64_t v_sb, int64_t v_sh, int64_t v_st, void* key_pages, void* value_pages,
+                    int64_t num_pages, int64_t page_size, const int64_t* pages, int64_t max_pages,
+                    const int64_t* lengths, int* bad_page_dev, void* stream);
+/* Positions [0, lengths[b]) of each sequence as contiguous (batch, kv_heads, longest, head_dim),
+ * zeros behind them; positions from `longest` on are left out. */
+int tg_paged_gather(int dtype, int64_t batch, int64_t longest, int64_t kv_heads, int64_t head_dim,
+                    const void* key_pages, const void* value_pages, int64_t num_pages,
+                    int64_t page_size, const int64_t* pages, int64_t max_pages,
+                    const int64_t* lengths, void* k, void* v, int* bad_page_dev, void* stream);
+/* Copies page src[i] to page dst[i] (int64, on the device) in every one of `layers` consecutive
+ * pools of num_pages pages of page_bytes (a multiple of 4) at key_pages and at value_pages. The
+ * dst pages are distinct and none of them is a src page. */
+int tg_page_copy(int64_t page_bytes, int64_t layers, int64_t num_pages, void* key_pages,
+                 void* value_pages, const int64_t* src, const int64_t* dst, int64_t pairs,
+                 int* bad_page_dev, void* stream);
+/* One new token's attention: out (batch, heads, head_dim), contiguous, = softmax(q k^T /
+ * sqrt(head_dim)) v over the sequence's first lengths[b] positions, query head h on key head
+ * h / (heads / kv_heads); lse (batch, heads; may be NULL) = the log-sum-exp of the scaled
+ * scores. An empty sequence gives zeros and -inf. head_dim <= 256. `longest`: about how long
+ * the longest sequence is (any positive value is right, a near one is fastest). `scratch`:
+ * tg_paged_attention_scratch_bytes of the same sizes. */
+size_t tg_paged_attention_scratch_bytes(int dtype, int64_t batch, int64_t heads, int64_t kv_heads,
+                                        int64_t head_dim, int64_t longest);
+int tg_paged_attention(int dtype, int64_t batch, int64_t heads, int64_t kv_heads,
+                       int64_t head_dim, const void* q, int64_t q_sb, int64_t q_sh,
+                       const void* key_pages, const void* value_pages, int64_t num_pages,
+                       int64_t page_size, const int64_t* pages, int64_t max_pages,
+                       const int64_t* lengths, int64_t longest, void* out, void* lse,
+                       int* bad_page_dev, void* scratch, void* stream);
+
 /* ------------------------------------------------------------------ convolution / pooling
  * conv2d (ops/conv.py:128-177): cross-correlation of x (n, c, h, w) with w (c_out, c, kh, kw)
  * by an im2col patch matrix `cols` stored patch-major: `rows` x `ld` from

@@ -159,6 +159,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tg_attention_backward_dropout": (c_int, [c_int, POINTER(AttnShape), vp, vp, vp, vp, vp, vp,
                                               vp, POINTER(ctypes.c_uint64), ctypes.c_uint32, dbl,
                                               vp, vp]),
+    "tg_paged_append": (c_int, [c_int, i64, i64, i64, i64, vp, i64, i64, i64, vp, i64, i64, i64,
+                                vp, vp, i64, i64, vp, i64, vp, vp, vp]),
+    "tg_paged_gather": (c_int, [c_int, i64, i64, i64, i64, vp, vp, i64, i64, vp, i64, vp, vp, vp,
+                                vp, vp]),
+    "tg_page_copy": (c_int, [i64, i64, i64, vp, vp, vp, vp, i64, vp, vp]),
+    "tg_paged_attention_scratch_bytes": (sz, [c_int, i64, i64, i64, i64, i64]),
+    "tg_paged_attention": (c_int, [c_int, i64, i64, i64, i64, vp, i64, i64, vp, vp, i64, i64, vp,
+                                   i64, vp, i64, vp, vp, vp, vp, vp]),
     "tg_conv2d_cols_shape": (c_int, [POINTER(ConvShape), pi64, pi64]),
     "tg_conv2d_forward_scratch_bytes": (sz, [c_int, POINTER(ConvShape)]),
     "tg_conv2d_forward": (c_int, [c_int, POINTER(ConvShape), vp, vp, vp, vp, vp, vp, vp]),

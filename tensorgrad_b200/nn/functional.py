@@ -8,3 +8,4 @@ from tensorgrad_b200.ops import (  # noqa: F401
 from tensorgrad_b200.ops.attention import (  # noqa: F401
     packed_self_attention, scaled_dot_product_attention,
 )
+from tensorgrad_b200.ops.paged import paged_attention  # noqa: F401

@@ -13,6 +13,7 @@ only the last position's logits come back to the host for sampling.
 from __future__ import annotations
 
 import math
+from collections.abc import Sequence
 from dataclasses import dataclass
 from typing import Any
 
@@ -24,10 +25,13 @@ from tensorgrad_b200.autograd import is_grad_enabled, no_grad
 from tensorgrad_b200.nn.attention import LayerCache, MultiHeadAttention
 from tensorgrad_b200.nn.layers import GELU, Dropout, Embedding, LayerNorm, Linear, Sequential
 from tensorgrad_b200.nn.module import Module
+from tensorgrad_b200.nn.paged import PagedBatch, PagedKVCache, PagedLayer
+from tensorgrad_b200.ops.loss import token_log_probs
+from tensorgrad_b200.ops.shape import concat
 from tensorgrad_b200.tensor import Tensor
 from tensorgrad_b200.utils.grad_checkpoint import checkpoint
 
-__all__ = ["GPT", "GPTConfig", "KVCache", "TransformerBlock"]
+__all__ = ["GPT", "GPTConfig", "KVCache", "Sampled", "TransformerBlock"]
 
 
 class TransformerBlock(Module):
@@ -44,7 +48,7 @@ class TransformerBlock(Module):
         self.mlp = Sequential(Linear(embed_dim, hidden), GELU(), Linear(hidden, embed_dim),
                               Dropout(dropout))
 
-    def forward(self, x: Tensor, cache: LayerCache | None = None) -> Tensor:
+    def forward(self, x: Tensor, cache: LayerCache | PagedLayer | None = None) -> Tensor:
         x = x + self.attn(self.ln1(x), cache)
         return x + self.mlp(self.ln2(x))
 
@@ -59,6 +63,15 @@ class KVCache:
     def length(self) -> int:
         """Positions already cached."""
         return self.layers[0].length if self.layers else 0
+
+
+@dataclass
+class Sampled:
+    """One continuation of :meth:`GPT.generate_batch`: the prompt's and the new ids, and the
+    new ids' log probabilities under the model (before temperature and top-k)."""
+
+    ids: np.ndarray
+    log_probs: np.ndarray
 
 
 @dataclass(frozen=True)
@@ -118,13 +131,16 @@ class GPT(Module):
                 bias.data.fill_(0.0)
 
     # ------------------------------------------------------------------ forward
-    def forward(self, idx: Any, cache: KVCache | None = None) -> Tensor:
+    def forward(self, idx: Any, cache: KVCache | PagedBatch | None = None) -> Tensor:
         """Logits for token ids ``(B, T)``; with a ``cache``, ids continue the cached ones
-        (positions from ``cache.length``; inference only, no graph). Host ids are checked
+        (positions from ``cache.length``, or each row's own length in a
+        ``PagedKVCache.batch``; inference only, no graph). Host ids are checked
         on the host; ids in a device tensor stay on the device (checked there)."""
         tokens = idx if isinstance(idx, Tensor) else np.asarray(idx)
         if tokens.ndim != 2:
             raise ValueError(f"expected (B, T) token ids, got shape {tokens.shape}")
+        if isinstance(cache, PagedBatch):
+            return self._forward_paged(tokens, cache)
         start = cache.length if cache is not None else 0
         t = tokens.shape[1]
         if start + t > self.config.block_size:
@@ -144,12 +160,93 @@ class GPT(Module):
                 x = block(x, layer)
             return self.head(self.ln_f(x))
 
+    def _forward_paged(self, tokens: Any, rows: PagedBatch) -> Tensor:
+        b, t = tokens.shape
+        starts = rows.lengths
+        if b != len(starts):
+            raise ValueError(f"{b} rows of ids for {len(starts)} sequences")
+        if t == 0:
+            raise ValueError("a step needs at least one token")
+        if int(starts.max()) + t > self.config.block_size:
+            raise ValueError(f"sequence length {int(starts.max()) + t} exceeds block_size "
+                             f"{self.config.block_size}")
+        if self.training:
+            raise ValueError("a KV cache is for inference: call eval() first")
+        rows.check_model(len(self.blocks), self.blocks[0].attn if len(self.blocks) else None,
+                         self.tok_emb.weight.dtype)
+        with no_grad():
+            steps = rows.begin(t)
+            x = self.tok_emb(tokens) + self.pos_emb(starts[:, None] + np.arange(t))
+            for block, layer in zip(self.blocks, steps, strict=True):
+                x = block(x, layer)
+            logits = self.head(self.ln_f(x))
+        rows.commit(t)
+        return logits
+
     # ------------------------------------------------------------------ generation
     def make_cache(self, batch_size: int) -> KVCache:
         """Empty per-layer device caches for ``batch_size`` sequences of ``block_size``."""
         dt = self.tok_emb.weight.dtype
         return KVCache([LayerCache.empty(batch_size, blk.attn.num_heads, self.config.block_size,
                                          blk.attn.head_dim, dt) for blk in self.blocks])
+
+    def make_paged_cache(self, num_pages: int, page_size: int = 16) -> PagedKVCache:
+        """An empty cache of ``num_pages`` pages of ``page_size`` positions for this model's
+        layers, to be shared by any number of sequences."""
+        attn = self.blocks[0].attn
+        return PagedKVCache(self.config.n_layer, attn.num_heads, attn.head_dim, num_pages,
+                            page_size, self.tok_emb.weight.dtype)
+
+    def generate_batch(self, prompts: Sequence[Any], max_new_tokens: int, *, samples: int = 1,
+                       temperature: float = 1.0, top_k: int | None = None,
+                       rng: np.random.Generator | None = None,
+                       page_size: int = 16) -> list[list[Sampled]]:
+        """``samples`` continuations of each prompt (1-D ids of any lengths, each at least
+        one) by ``max_new_tokens`` sampled tokens, all in one batch over a paged cache: a
+        prompt is encoded once and forked, every step then costs one position per
+        continuation. Prompts and new tokens have to fit in ``block_size``. Sampling is
+        :meth:`generate`'s, row by row in the order of the result."""
+        if temperature <= 0:
+            raise ValueError("temperature must be positive")
+        if samples < 1 or max_new_tokens < 0:
+            raise ValueError(f"cannot draw {samples} samples of {max_new_tokens} tokens")
+        texts = [np.asarray(p, dtype=np.int64) for p in prompts]
+        for p in texts:
+            if p.ndim != 1 or p.size == 0:
+                raise ValueError(f"expected prompts of at least one id, got shape {p.shape}")
+            if p.size + max_new_tokens > self.config.block_size:
+                raise ValueError(f"sequence length {p.size + max_new_tokens} exceeds block_size "
+                                 f"{self.config.block_size}")
+        if not texts:
+            return []
+        gen = rng or get_rng()
+        was_training = self.training
+        self.eval()
+        most = sum(-(-(p.size + max_new_tokens) // page_size) for p in texts) * samples
+        ids = [p for p in texts for _ in range(samples)]
+        scores: list[list[np.ndarray]] = [[] for _ in ids]
+        try:
+            cache = self.make_paged_cache(most, page_size)
+            rows: list[int] = []
+            firsts = []
+            for p in texts if max_new_tokens else ():
+                seq = cache.add()
+                firsts.append(self(p[None], cache=cache.batch([seq]))[:, -1])
+                rows += [seq, *(cache.fork(seq) for _ in range(samples - 1))]
+            logits = concat([f for f in firsts for _ in range(samples)]) if firsts else None
+            for step in range(max_new_tokens):
+                new = _sample(logits.numpy().astype(np.float64) / temperature, top_k, gen)
+                found = token_log_probs(logits, new).log_probs.numpy()
+                for i, token in enumerate(new):
+                    ids[i] = np.append(ids[i], token)
+                    scores[i].append(found[i])
+                if step + 1 < max_new_tokens:
+                    logits = self(new[:, None], cache=cache.batch(rows))[:, -1]
+        finally:
+            self.train(was_training)
+        out = [Sampled(i, np.array(s, dtype=self.tok_emb.weight.dtype))
+               for i, s in zip(ids, scores, strict=True)]
+        return [out[k:k + samples] for k in range(0, len(out), samples)]
 
     def generate(self, idx: Any, max_new_tokens: int, *, temperature: float = 1.0,
                  top_k: int | None = None, rng: np.random.Generator | None = None,

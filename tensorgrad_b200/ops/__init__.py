@@ -12,6 +12,7 @@ from tensorgrad_b200.ops.linalg import matmul
 from tensorgrad_b200.ops.loss import (
     TokenLogProbs, binary_cross_entropy_with_logits, cross_entropy, mse_loss, token_log_probs,
 )
+from tensorgrad_b200.ops.paged import append_pages, copy_pages, gather_pages, paged_attention
 from tensorgrad_b200.ops.recurrent import gru, lstm, rnn
 from tensorgrad_b200.ops.reduce import max, mean, min, sum, var
 from tensorgrad_b200.ops.shape import (
@@ -20,11 +21,11 @@ from tensorgrad_b200.ops.shape import (
 )
 
 __all__ = [
-    "TokenLogProbs", "add", "astype", "batch_norm", "binary_cross_entropy_with_logits", "broadcast_to", "concat",
-    "conv2d", "cross_entropy", "div", "dropout", "embedding", "exp", "flatten", "gelu", "getitem",
+    "TokenLogProbs", "add", "append_pages", "astype", "batch_norm", "binary_cross_entropy_with_logits", "broadcast_to", "concat",
+    "conv2d", "cross_entropy", "div", "dropout", "embedding", "exp", "flatten", "gather_pages", "gelu", "getitem",
     "gru", "layer_norm", "linear", "log", "log_softmax", "logsumexp", "lstm", "masked_fill",
     "matmul", "max", "max_pool2d", "mean", "min", "mse_loss", "mul", "neg",
-    "packed_self_attention", "permute", "pow", "relu", "reshape", "rnn",
+    "packed_self_attention", "paged_attention", "permute", "pow", "relu", "reshape", "rnn",
     "scaled_dot_product_attention", "sigmoid", "softmax", "sqrt", "squeeze", "stack", "sub",
     "sum", "sum_to", "tanh", "token_log_probs", "transpose", "unsqueeze", "var", "where",
 ]
