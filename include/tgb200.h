@@ -394,6 +394,23 @@ int tg_attention_backward_dropout(int dtype, const tg_attn_shape* s, const void*
                                   uint32_t threshold, double keep_scale, void* scratch,
                                   void* stream);
 
+/* ------------------------------------------------------------------ 8-bit integer linear
+ * The inference form of ops/layers.py:22-62 with a scale for each token and each channel (no
+ * reference counterpart). tg_int8_quantize_rows: scales[r] = max|x[r]| / 127, q[r][c] = the
+ * nearest integer to x[r][c] / scales[r] (halves to even, quotient rounded to the type first),
+ * rows of ld >= inner bytes with zeros behind the values. A row of zeros has scale 0 and
+ * integers 0, a row with a NaN or an infinity scale NaN and integers 0. */
+int tg_int8_quantize_rows(int dtype, const void* x, int64_t rows, int64_t inner, int8_t* q,
+                          int64_t ld, void* scales, void* stream);
+/* y (rows, outer) = (q(x) w^T) (scale of the row * scales[channel]) + bias (may be NULL), the
+ * integer sums exact. weight: (outer, ld) int8 on a 16-byte boundary, ld >= inner a multiple of
+ * 16; its bytes behind inner do not count. inner <= 131072. x, scales, bias and y have `dtype`.
+ * `scratch`: tg_int8_linear_scratch_bytes of the same sizes. */
+size_t tg_int8_linear_scratch_bytes(int dtype, int64_t rows, int64_t inner, int64_t outer);
+int tg_int8_linear(int dtype, const void* x, int64_t rows, int64_t inner, const int8_t* weight,
+                   int64_t ld, const void* scales, const void* bias, void* y, int64_t outer,
+                   void* scratch, void* stream);
+
 /* ------------------------------------------------------------------ paged key-value cache
  * The cache of nn/attention.py:27-111 in pages, so that sequences of different lengths share
  * one pool and prefixes (no reference counterpart). key_pages and value_pages each hold

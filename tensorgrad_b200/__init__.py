@@ -11,12 +11,12 @@ from tensorgrad_b200._random import get_rng, manual_seed
 from tensorgrad_b200.autograd import enable_grad, is_grad_enabled, no_grad
 from tensorgrad_b200.device import DeviceArray, set_device, synchronize
 from tensorgrad_b200.ops import (
-    add, append_pages, binary_cross_entropy_with_logits, broadcast_to, concat, conv2d, copy_pages, cross_entropy, div,
-    dropout, embedding, exp, flatten, gather_pages, gelu, layer_norm, linear, log, log_softmax, logsumexp,
-    masked_fill, matmul, max, max_pool2d, mean, min, mse_loss, mul, neg, paged_attention, permute, pow, relu,
-    reshape, sigmoid, softmax, sqrt, squeeze, stack, sub, sum, tanh,
-    token_log_probs, transpose, unsqueeze, var,
-    where,
+    Int8Weight, add, append_pages, binary_cross_entropy_with_logits, broadcast_to, concat,
+    conv2d, copy_pages, cross_entropy, div, dropout, embedding, exp, flatten, gather_pages,
+    gelu, int8_linear, layer_norm, linear, log, log_softmax, logsumexp, masked_fill, matmul,
+    max, max_pool2d, mean, min, mse_loss, mul, neg, paged_attention, permute, pow,
+    quantize_int8, relu, reshape, sigmoid, softmax, sqrt, squeeze, stack, sub, sum, tanh,
+    token_log_probs, transpose, unsqueeze, var, where,
 )
 from tensorgrad_b200.tensor import (
     Tensor, arange, full, get_default_dtype, ones, ones_like, rand, randn, set_default_dtype,
@@ -35,15 +35,15 @@ def _lib_launches() -> int:
     return int(lib.tg_launch_count())
 
 __all__ = [
-    "DeviceArray", "Tensor", "__version__", "add", "append_pages", "arange", "autograd",
-    "binary_cross_entropy_with_logits", "broadcast_to", "concat", "conv2d", "copy_pages",
-    "cross_entropy",
-    "div", "dropout", "embedding", "enable_grad", "exp", "flatten", "full", "func", "gather_pages", "gelu",
-    "get_default_dtype", "get_rng", "is_grad_enabled", "layer_norm", "linear", "log",
-    "log_softmax", "logsumexp", "manual_seed", "masked_fill", "matmul", "max", "max_pool2d",
-    "mean", "min", "mse_loss", "mul", "neg", "nn", "no_grad", "ones", "ones_like", "optim",
-    "paged_attention", "permute", "pow", "profiler", "rand", "randn", "relu", "reshape", "set_default_dtype",
-    "set_device", "sigmoid", "softmax", "sqrt", "squeeze", "stack", "sub", "sum", "synchronize",
-    "tanh", "tensor", "token_log_probs", "transpose", "unsqueeze", "utils", "var", "viz", "where", "zeros",
-    "zeros_like",
+    "DeviceArray", "Int8Weight", "Tensor", "__version__", "add", "append_pages", "arange",
+    "autograd", "binary_cross_entropy_with_logits", "broadcast_to", "concat", "conv2d",
+    "copy_pages", "cross_entropy", "div", "dropout", "embedding", "enable_grad", "exp",
+    "flatten", "full", "func", "gather_pages", "gelu", "get_default_dtype", "get_rng",
+    "int8_linear", "is_grad_enabled", "layer_norm", "linear", "log", "log_softmax",
+    "logsumexp", "manual_seed", "masked_fill", "matmul", "max", "max_pool2d", "mean", "min",
+    "mse_loss", "mul", "neg", "nn", "no_grad", "ones", "ones_like", "optim",
+    "paged_attention", "permute", "pow", "profiler", "quantize_int8", "rand", "randn", "relu",
+    "reshape", "set_default_dtype", "set_device", "sigmoid", "softmax", "sqrt", "squeeze",
+    "stack", "sub", "sum", "synchronize", "tanh", "tensor", "token_log_probs", "transpose",
+    "unsqueeze", "utils", "var", "viz", "where", "zeros", "zeros_like",
 ]

@@ -159,6 +159,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tg_attention_backward_dropout": (c_int, [c_int, POINTER(AttnShape), vp, vp, vp, vp, vp, vp,
                                               vp, POINTER(ctypes.c_uint64), ctypes.c_uint32, dbl,
                                               vp, vp]),
+    "tg_int8_quantize_rows": (c_int, [c_int, vp, i64, i64, vp, i64, vp, vp]),
+    "tg_int8_linear_scratch_bytes": (sz, [c_int, i64, i64, i64]),
+    "tg_int8_linear": (c_int, [c_int, vp, i64, i64, vp, i64, vp, vp, vp, i64, vp, vp]),
     "tg_paged_append": (c_int, [c_int, i64, i64, i64, i64, vp, i64, i64, i64, vp, i64, i64, i64,
                                 vp, vp, i64, i64, vp, i64, vp, vp, vp]),
     "tg_paged_gather": (c_int, [c_int, i64, i64, i64, i64, vp, vp, i64, i64, vp, i64, vp, vp, vp,

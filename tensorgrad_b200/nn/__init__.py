@@ -3,8 +3,8 @@
 from tensorgrad_b200.nn import functional, init
 from tensorgrad_b200.nn.attention import LayerCache, MultiHeadAttention
 from tensorgrad_b200.nn.layers import (
-    GELU, MLP, BatchNorm1d, BatchNorm2d, Conv2d, Dropout, Embedding, Flatten, Identity, LayerNorm,
-    Linear, MaxPool2d, ReLU, Sequential, Sigmoid, Tanh,
+    GELU, MLP, BatchNorm1d, BatchNorm2d, Conv2d, Dropout, Embedding, Flatten, Identity,
+    Int8Linear, LayerNorm, Linear, MaxPool2d, ReLU, Sequential, Sigmoid, Tanh,
 )
 from tensorgrad_b200.nn.module import IncompatibleKeys, Module, Parameter
 from tensorgrad_b200.nn.paged import PagedBatch, PagedKVCache
@@ -13,7 +13,7 @@ from tensorgrad_b200.nn.transformer import GPT, GPTConfig, KVCache, Sampled, Tra
 
 __all__ = [
     "GELU", "GPT", "GRU", "LSTM", "MLP", "BatchNorm1d", "BatchNorm2d", "Conv2d", "Dropout", "Embedding",
-    "Flatten", "GPTConfig", "Identity", "IncompatibleKeys", "KVCache", "LayerCache", "LayerNorm",
+    "Flatten", "GPTConfig", "Identity", "IncompatibleKeys", "Int8Linear", "KVCache", "LayerCache", "LayerNorm",
     "Linear", "MaxPool2d",
     "Module", "MultiHeadAttention", "PagedBatch", "PagedKVCache", "Parameter", "RNN", "ReLU",
     "Sampled", "Sequential", "Sigmoid", "Tanh",

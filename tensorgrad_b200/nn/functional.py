@@ -2,7 +2,7 @@
 
 from tensorgrad_b200.ops import (  # noqa: F401
     batch_norm, binary_cross_entropy_with_logits, conv2d, cross_entropy, dropout, embedding,
-    gelu, gru, layer_norm, linear, log_softmax, lstm, max_pool2d, mse_loss, relu, rnn, sigmoid,
+    gelu, gru, int8_linear, layer_norm, linear, log_softmax, lstm, max_pool2d, mse_loss, relu, rnn, sigmoid,
     softmax, tanh, token_log_probs,
 )
 from tensorgrad_b200.ops.attention import (  # noqa: F401

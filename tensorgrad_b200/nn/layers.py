@@ -20,7 +20,7 @@ from tensorgrad_b200.nn.module import Module, Parameter
 from tensorgrad_b200.tensor import Tensor, get_default_dtype
 
 __all__ = ["GELU", "MLP", "BatchNorm1d", "BatchNorm2d", "Conv2d", "Dropout", "Embedding",
-           "Flatten", "Identity", "LayerNorm", "Linear", "MaxPool2d", "ReLU", "Sequential",
+           "Flatten", "Identity", "Int8Linear", "LayerNorm", "Linear", "MaxPool2d", "ReLU", "Sequential",
            "Sigmoid", "Tanh"]
 
 
@@ -52,6 +52,29 @@ class Linear(Module):
 
     def extra_repr(self) -> str:
         return f"{self.in_features}, {self.out_features}, bias={self.bias is not None}"
+
+
+class Int8Linear(Module):
+    """A :class:`Linear` for inference with its weight in 8-bit integers, a scale for each
+    output channel, and its input quantised token by token in the call (no counterpart in the
+    reference). Made from a trained layer; integers, scales and bias are buffers."""
+
+    def __init__(self, linear: Linear) -> None:
+        super().__init__()
+        self.in_features, self.out_features = linear.in_features, linear.out_features
+        quantized = ops.Int8Weight.quantize(linear.weight)
+        self.register_buffer("weight", quantized.q)
+        self.register_buffer("scale", quantized.scale)
+        self.has_bias = linear.bias is not None
+        if linear.bias is not None:
+            self.register_buffer("bias", linear.bias.data.copy())
+
+    def forward(self, x: Tensor) -> Tensor:
+        weight = ops.Int8Weight(self.weight, self.scale, self.in_features)
+        return ops.int8_linear(x, weight, Tensor._wrap(self.bias) if self.has_bias else None)
+
+    def extra_repr(self) -> str:
+        return f"{self.in_features}, {self.out_features}, bias={self.has_bias}"
 
 
 class Conv2d(Module):

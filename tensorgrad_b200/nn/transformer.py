@@ -23,7 +23,9 @@ from tensorgrad_b200 import device
 from tensorgrad_b200._random import get_rng
 from tensorgrad_b200.autograd import is_grad_enabled, no_grad
 from tensorgrad_b200.nn.attention import LayerCache, MultiHeadAttention
-from tensorgrad_b200.nn.layers import GELU, Dropout, Embedding, LayerNorm, Linear, Sequential
+from tensorgrad_b200.nn.layers import (
+    GELU, Dropout, Embedding, Int8Linear, LayerNorm, Linear, Sequential,
+)
 from tensorgrad_b200.nn.module import Module
 from tensorgrad_b200.nn.paged import PagedBatch, PagedKVCache, PagedLayer
 from tensorgrad_b200.ops.loss import token_log_probs
@@ -129,6 +131,23 @@ class GPT(Module):
             bias = getattr(module, "bias", None)
             if bias is not None:
                 bias.data.fill_(0.0)
+
+    def quantize_int8(self, head: bool = False) -> GPT:
+        """Turn this model into one for inference whose blocks' linear layers (and with
+        ``head`` the vocabulary head) hold their weights in 8-bit integers
+        (:class:`Int8Linear`). The other parameters stop requiring gradients; a tied
+        embedding keeps its floating table."""
+        for block in self.blocks:
+            for parent, name in ((block.attn, "qkv"), (block.attn, "proj"), (block.mlp, "0"),
+                                 (block.mlp, "2")):
+                layer = getattr(parent, name)
+                if isinstance(layer, Linear):
+                    setattr(parent, name, Int8Linear(layer))
+        if head and isinstance(self.head, Linear):
+            self.head = Int8Linear(self.head)
+        for p in self.parameters():
+            p.requires_grad = False
+        return self.eval()
 
     # ------------------------------------------------------------------ forward
     def forward(self, idx: Any, cache: KVCache | PagedBatch | None = None) -> Tensor:

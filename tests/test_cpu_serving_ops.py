@@ -261,3 +261,60 @@ def test_paged_cache_refusals_and_sharing(monkeypatch):
         with pytest.raises(ValueError, match="must be positive"):
             _Books.make(monkeypatch, **{**dict(layers=1, kv_heads=1, head_dim=1, num_pages=1,
                                                page_size=1), **bad})
+
+
+# ---------------------------------------------------------------------- 8-bit integers
+def _weight(outer, inner, dtype=np.float32):
+    from tensorgrad_b200.ops import Int8Weight
+
+    w = Int8Weight.__new__(Int8Weight)
+    w.q, w.scale, w.in_features = _Meta((outer, -(-inner // 16) * 16), np.int8), _Meta((outer,), dtype), inner
+    return w
+
+
+def test_int8_ops_refuse_bad_arguments():
+    from tensorgrad_b200.ops import Int8Weight, int8_linear, quantize_int8
+
+    with pytest.raises(TypeError, match="takes an Int8Weight"):
+        int8_linear(_t((2, 8)), _t((4, 8)))
+    for shape in ((2, 7), ()):
+        with pytest.raises(ValueError, match="does not match weight"):
+            int8_linear(_t(shape), _weight(4, 8))
+    with pytest.raises(TypeError, match="int64"):
+        int8_linear(_t((2, 8), np.int64), _weight(4, 8))
+    with pytest.raises(ValueError, match=r"bias \(3,\) for 4"):
+        int8_linear(_t((2, 8)), _weight(4, 8), _t((3,)))
+    learnt = _t((2, 8))
+    learnt._requires_grad = True
+    with pytest.raises(ValueError, match="inference"):
+        int8_linear(learnt, _weight(4, 8))
+    for shape in ((), (3, 0)):
+        with pytest.raises(ValueError, match="last axis"):
+            quantize_int8(_t(shape))
+    with pytest.raises(TypeError, match="expected int8"):
+        Int8Weight(_t((4, 16), np.float32), _t((4,)))
+    with pytest.raises(TypeError, match="expected int8"):
+        Int8Weight(_t((16,), np.int8), _t((4,)))
+    for inner in (0, 17):
+        with pytest.raises(ValueError, match=r"in_features must be in \[1, 16\]"):
+            Int8Weight(_t((4, 16), np.int8), _t((4,)), inner)
+    with pytest.raises(ValueError, match="4 floating scales"):
+        Int8Weight(_t((4, 16), np.int8), _t((3,)))
+    with pytest.raises(ValueError, match="4 floating scales"):
+        Int8Weight(_t((4, 16), np.int8), _t((4,), np.int64))
+    with pytest.raises(ValueError, match="expected a weight"):
+        Int8Weight.quantize(_t((4,)))
+
+
+def test_int8_entry_points_refuse_bad_sizes():
+    from tensorgrad_b200._lib import lib
+
+    def linear(rows=2, inner=20, ld=32, outer=3, dtype=0, scratch=None):
+        return lib.tg_int8_linear(dtype, None, rows, inner, None, ld, None, None, None, outer,
+                                  scratch, None)
+
+    assert linear(rows=0) == 0 and linear(outer=0) == 0
+    for bad in (dict(rows=-1), dict(inner=0), dict(ld=16), dict(ld=40), dict(outer=-1), dict()):
+        assert linear(**bad) == 1, bad
+    assert linear(inner=131073, ld=131088) == 3
+    assert lib.tg_int8_quantize_rows(0, None, 1, 20, None, 19, None, None) == 1
