@@ -107,57 +107,401 @@ page_copy_kernel(V* keys, V* values, int64_t layers, int64_t num_pages, int64_t 
 
 // ---------------------------------------------------------------- attention of one token
 constexpr int kMaxHead = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kLaneDims = 8;        // features of a position that one lane holds
+constexpr int kTable = 2048;        // pages named in shared memory at a time
+constexpr int kMinSplit = 256;      // positions that a block has at least, if there are as many
+constexpr int kMaxSplits = 512;
 
-// One block per (sequence, query head): each warp walks every eighth position with its own
-// running maximum, sum and output, the eight are joined at the end.
+// n / d for 0 <= n < 2^31 by a multiplication (d fixed for a launch; Granlund and Montgomery,
+// "Division by invariant integers using multiplication", 1994).
+struct FastDiv {
+  uint32_t d, mul, shift;
+};
+FastDiv make_div(int64_t d) {
+  uint32_t l = 0;
+  while (((int64_t)1 << l) < d) ++l;
+  return {(uint32_t)d, (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << l) - d)) / d + 1), l};
+}
+__device__ __forceinline__ int div_by(int n, FastDiv f) {
+  return (int)((__umulhi((uint32_t)n, f.mul) + (uint32_t)n) >> f.shift);
+}
+
+// e^x on scores that carry the factor `unit`: float scores are in base 2 (one instruction less
+// per weight), double ones in base e.
+template <typename T>
+struct Base;
+template <>
+struct Base<float> {
+  static constexpr double unit = 1.4426950408889634;  // log2 e
+  static __device__ __forceinline__ float exp_(float x) { return exp2f(x); }
+  static __device__ __forceinline__ float natural(float x) { return x * 0.6931471805599453f; }
+};
+template <>
+struct Base<double> {
+  static constexpr double unit = 1.0;
+  static __device__ __forceinline__ double exp_(double x) { return exp(x); }
+  static __device__ __forceinline__ double natural(double x) { return x; }
+};
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from, bool live) {
+  const int n = live ? BYTES : 0;  // nothing read, zeros written
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(n));
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES),
+                 "r"(n));
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+struct AttendArgs {
+  Pool pool;
+  int64_t heads, group, head_groups;  // query heads; to a key head; blocks that share one
+  int64_t q_sb, q_sh;
+  const int64_t* lengths;
+  int splits;
+  FastDiv size;
+  double scale;
+};
+
+// Positions to a split of a sequence of n: as even as `splits` makes them, but no fewer than
+// kMinSplit, in multiples of 32.
+__device__ __forceinline__ int split_length(int n, int splits) {
+  const int even = (n + splits - 1) / splits;
+  const int c = even > kMinSplit ? even : kMinSplit;
+  return (c + 31) / 32 * 32;
+}
+
+// One block per (sequence, key head, split of its positions, group of GH query heads). LPT lanes
+// share a position, each with 8 of its features, so a warp has 32 / LPT positions at a time and
+// every lane group runs its own softmax; queries and outputs of GH heads stay in registers. Each
+// lane copies its features of the next ST positions' keys and values into shared memory itself
+// (cp.async, VE elements at a time) and is the only one to read them: no barrier in the loop.
+// What bounds it: reading keys and values once. 2 blocks of 256 lanes keep up to 160 KB a
+// multiprocessor in flight.
+template <typename T, int VE, int LPT, int GH>
+struct Attend {
+  static constexpr int NVEC = kLaneDims / VE;
+  static constexpr int VB = VE * (int)sizeof(T);
+  static constexpr int STAGE = 2 * NVEC * VB * kThreads;
+  static constexpr int ST = sizeof(T) == 4 ? 6 : 3;
+  static constexpr int WIDTH = LPT * kLaneDims;  // features covered
+  static constexpr int RING = ST * STAGE;
+  static constexpr int JOIN = kWarps * GH * (WIDTH + 2) * (int)sizeof(T);
+  static constexpr int SMEM = (RING > JOIN ? RING : JOIN) + kTable * 4;
+};
+
+template <typename T, int VE, int LPT, int GH>
+__global__ void __launch_bounds__(kThreads, GH == 8 ? 1 : 2)
+paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restrict__ keys,
+                       const T* __restrict__ values, T* __restrict__ out, T* __restrict__ lse,
+                       T* __restrict__ part) {
+  using A = Attend<T, VE, LPT, GH>;
+  constexpr int NVEC = A::NVEC, ST = A::ST, TPW = 32 / LPT, STEP = kWarps * TPW;
+  extern __shared__ __align__(16) uint8_t smem[];
+  int* table = reinterpret_cast<int*>(smem + A::SMEM - kTable * 4);
+  pdl_trigger();
+  pdl_wait();
+  int64_t e = blockIdx.x;
+  const int64_t g0 = (e % a.head_groups) * GH;
+  e /= a.head_groups;
+  const int split = (int)(e % a.splits);
+  e /= a.splits;
+  const int64_t kh = e % a.pool.kv_heads, b = e / a.pool.kv_heads;
+  const int d = (int)a.pool.head_dim;
+  const int n = (int)length_of(a.pool, a.lengths, b);
+  const int len = split_length(n, a.splits);
+  const int begin = split * len, end = begin + len < n ? begin + len : n;
+  if (begin >= n && split > 0) return;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int sub = lane / LPT, j = lane % LPT;
+  const int64_t h0 = kh * a.group + g0;
+  const int live_heads = (int)(a.group - g0 < GH ? a.group - g0 : GH);
+
+  T qr[GH][kLaneDims], acc[GH][kLaneDims], m[GH], l[GH];
+#pragma unroll
+  for (int g = 0; g < GH; ++g) {
+    m[g] = T(-INFINITY);
+    l[g] = T(0);
+#pragma unroll
+    for (int i = 0; i < kLaneDims; ++i) {
+      const int c = ((i / VE) * LPT + j) * VE + i % VE;
+      qr[g][i] = g < live_heads && c < d
+                     ? q[b * a.q_sb + (h0 + g) * a.q_sh + c] * (T)(a.scale * Base<T>::unit)
+                     : T(0);
+      acc[g][i] = T(0);
+    }
+  }
+  const uint32_t ring =
+      (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * A::VB;
+  const uint8_t* mine = smem + threadIdx.x * A::VB;
+  // Features behind the head's width are never copied: they stay zero.
+  for (int i = 0; i < ST * 2 * NVEC; ++i) {
+    if (((i % NVEC) * LPT + j) * VE < d) continue;
+    T* z = reinterpret_cast<T*>(smem + threadIdx.x * A::VB + i * (A::VB * kThreads));
+#pragma unroll
+    for (int v = 0; v < VE; ++v) z[v] = T(0);
+  }
+  const int64_t page_rows = a.pool.kv_heads * a.pool.page_size;
+  for (int t0 = begin; t0 < end;) {
+    // The pages of the next positions, as many as the table holds.
+    const int p0 = div_by(t0, a.size);
+    const int64_t stop = (int64_t)(p0 + kTable) * a.size.d;
+    const int t1 = stop < end ? (int)stop : end;
+    const int used = div_by(t1 - 1, a.size) - p0 + 1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < used; i += kThreads) {
+      int64_t page = a.pool.table[b * a.pool.max_pages + p0 + i];
+      if (page < 0 || page >= a.pool.num_pages) {
+        if (a.pool.bad) *a.pool.bad = 1;
+        page = 0;
+      }
+      table[i] = (int)page;
+    }
+    __syncthreads();
+    const int steps = (t1 - t0 + STEP - 1) / STEP;
+    auto issue = [&](int i) {
+      const int t = t0 + i * STEP + w * TPW + sub;
+      const bool live = i < steps && t < t1;
+      int64_t at = 0;
+      if (live) {
+        const int p = div_by(t, a.size);
+        at = (table[p - p0] * page_rows + kh * a.pool.page_size + (t - p * (int)a.size.d)) * d;
+      }
+      const uint32_t to = ring + (i % ST) * A::STAGE;
+#pragma unroll
+      for (int v = 0; v < NVEC; ++v) {
+        const int c = (v * LPT + j) * VE;
+        if (c < d) {
+          copy_async<A::VB>(to + v * (A::VB * kThreads), keys + at + c, live);
+          copy_async<A::VB>(to + (NVEC + v) * (A::VB * kThreads), values + at + c, live);
+        }
+      }
+      copy_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i) issue(i);
+    for (int i = 0; i < steps; ++i) {
+      copy_wait<ST - 2>();
+      const uint8_t* from = mine + (i % ST) * A::STAGE;
+      T x[kLaneDims], s[GH];
+#pragma unroll
+      for (int v = 0; v < NVEC; ++v)
+#pragma unroll
+        for (int u = 0; u < VE; ++u)
+          x[v * VE + u] = reinterpret_cast<const T*>(from + v * (A::VB * kThreads))[u];
+#pragma unroll
+      for (int g = 0; g < GH; ++g) {
+        s[g] = T(0);
+#pragma unroll
+        for (int c = 0; c < kLaneDims; ++c) s[g] += qr[g][c] * x[c];
+      }
+#pragma unroll
+      for (int o = LPT / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int g = 0; g < GH; ++g) s[g] += __shfl_xor_sync(0xffffffffu, s[g], o);
+#pragma unroll
+      for (int v = 0; v < NVEC; ++v)
+#pragma unroll
+        for (int u = 0; u < VE; ++u)
+          x[v * VE + u] = reinterpret_cast<const T*>(from + (NVEC + v) * (A::VB * kThreads))[u];
+      const bool live = t0 + i * STEP + w * TPW + sub < t1;
+#pragma unroll
+      for (int g = 0; g < GH; ++g) {
+        if (!live || s[g] == T(-INFINITY)) continue;
+        if (s[g] > m[g]) {
+          const T c = Base<T>::exp_(m[g] - s[g]);
+          m[g] = s[g];
+          l[g] *= c;
+#pragma unroll
+          for (int k = 0; k < kLaneDims; ++k) acc[g][k] *= c;
+        }
+        const T p = Base<T>::exp_(s[g] - m[g]);
+        l[g] += p;
+#pragma unroll
+        for (int k = 0; k < kLaneDims; ++k) acc[g][k] += p * x[k];
+      }
+      issue(i + ST - 1);
+    }
+    copy_wait<0>();
+    t0 = t1;
+  }
+
+  // The warp's lane groups, then the block's warps.
+#pragma unroll
+  for (int o = LPT; o < 32; o <<= 1)
+#pragma unroll
+    for (int g = 0; g < GH; ++g) {
+      const T om = __shfl_xor_sync(0xffffffffu, m[g], o), mx = fmax(m[g], om);
+      const T c = l[g] == T(0) ? T(0) : Base<T>::exp_(m[g] - mx);
+      l[g] *= c;
+      l[g] += __shfl_xor_sync(0xffffffffu, l[g], o);
+      m[g] = mx;
+#pragma unroll
+      for (int k = 0; k < kLaneDims; ++k) {
+        acc[g][k] *= c;
+        acc[g][k] += __shfl_xor_sync(0xffffffffu, acc[g][k], o);
+      }
+    }
+  __syncthreads();
+  T* sacc = reinterpret_cast<T*>(smem);                // [warp][GH][WIDTH]
+  T* sm = sacc + kWarps * GH * A::WIDTH;               // [warp][GH]
+  T* sl = sm + kWarps * GH;
+  if (sub == 0) {
+#pragma unroll
+    for (int g = 0; g < GH; ++g) {
+#pragma unroll
+      for (int k = 0; k < kLaneDims; ++k)
+        sacc[(w * GH + g) * A::WIDTH + ((k / VE) * LPT + j) * VE + k % VE] = acc[g][k];
+      if (j == 0) {
+        sm[w * GH + g] = m[g];
+        sl[w * GH + g] = l[g];
+      }
+    }
+  }
+  __syncthreads();
+  const bool whole = n <= len;  // no other split of this sequence
+  for (int i = threadIdx.x; i < live_heads * d; i += kThreads) {
+    const int g = i / d, c = i % d;
+    T mx = T(-INFINITY), sum = T(0), v = T(0);
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) mx = fmax(mx, sm[k * GH + g]);
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) {
+      const T ls = sl[k * GH + g];
+      const T f = ls == T(0) ? T(0) : Base<T>::exp_(sm[k * GH + g] - mx);
+      sum += ls * f;
+      v += (ls == T(0) ? T(0) : sacc[(k * GH + g) * A::WIDTH + c]) * f;
+    }
+    const int64_t head = b * a.heads + h0 + g;
+    if (whole) {
+      out[head * d + c] = n == 0 ? T(0) : v / sum;
+      if (c == 0 && lse)
+        lse[head] = n == 0 ? T(-INFINITY) : Base<T>::natural(mx) + dev_log<T>(sum);
+    } else {
+      T* to = part + (head * a.splits + split) * (d + 2);
+      to[2 + c] = v;
+      if (c == 0) {
+        to[0] = mx;
+        to[1] = sum;
+      }
+    }
+  }
+}
+
+// The splits of a sequence's head as one: block per (sequence, head), the splits dealt to the
+// warps.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-paged_attention_kernel(Pool p, int64_t heads, const T* __restrict__ q, int64_t q_sb, int64_t q_sh,
-                       const T* __restrict__ keys, const T* __restrict__ values,
-                       const int64_t* __restrict__ lengths, T scale, T* __restrict__ out,
-                       T* __restrict__ lse) {
-  constexpr int W = kThreads / 32, N = kMaxHead / 32;
-  __shared__ T sm[W], sl[W], sa[W][kMaxHead];
-  const int64_t b = blockIdx.x / heads, h = blockIdx.x % heads;
-  const int64_t kh = h / (heads / p.kv_heads);
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int d = (int)p.head_dim;
-  const int64_t n = length_of(p, lengths, b);
-  T qr[N], acc[N], m = T(-INFINITY), l = T(0);
+paged_join_kernel(AttendArgs a, const T* __restrict__ part, T* __restrict__ out,
+                  T* __restrict__ lse) {
+  constexpr int N = kMaxHead / 32;
+  __shared__ T sacc[kWarps][kMaxHead], sl[kWarps];
+  pdl_wait();
+  const int64_t head = blockIdx.x, b = head / a.heads;
+  const int d = (int)a.pool.head_dim, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int n = (int)length_of(a.pool, a.lengths, b);
+  const int len = split_length(n, a.splits);
+  if (n <= len) return;  // written by its only block
+  const int live = (n + len - 1) / len;
+  const T* from = part + head * a.splits * (d + 2);
+  T mx = T(-INFINITY);
+  for (int i = lane; i < live; i += 32) mx = fmax(mx, from[(int64_t)i * (d + 2)]);
+  mx = warp_max(mx);
+  T acc[N] = {}, sum = T(0);
+  for (int i = w; i < live; i += kWarps) {
+    const T* p = from + (int64_t)i * (d + 2);
+    const T ls = p[1], f = ls == T(0) ? T(0) : Base<T>::exp_(p[0] - mx);
+    sum += ls * f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    qr[i] = lane + 32 * i < d ? q[b * q_sb + h * q_sh + lane + 32 * i] * scale : T(0);
-    acc[i] = T(0);
+    for (int k = 0; k < N; ++k)
+      if (lane + 32 * k < d) acc[k] += p[2 + lane + 32 * k] * f;
   }
-  for (int64_t t = w; t < n; t += W) {
-    int64_t at = row_of(p, b, kh, t);
-    if (at < 0) at = kh * p.page_size * p.head_dim;
-    T s = T(0);
+  if (lane == 0) sl[w] = sum;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (lane + 32 * i < d) s += qr[i] * keys[at + lane + 32 * i];
-    s = warp_sum(s);
-    const T mn = fmax(m, s), c = m == mn ? T(1) : dev_exp<T>(m - mn);
-    const T e = s == T(-INFINITY) ? T(0) : dev_exp<T>(s - mn);
-    l = l * c + e;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (lane + 32 * i < d) acc[i] = acc[i] * c + e * values[at + lane + 32 * i];
-    m = mn;
-  }
-  if (lane == 0) { sm[w] = m; sl[w] = l; }
-#pragma unroll
-  for (int i = 0; i < N; ++i) sa[w][lane + 32 * i] = acc[i];
+  for (int k = 0; k < N; ++k) sacc[w][lane + 32 * k] = acc[k];
   __syncthreads();
-  T mx = T(-INFINITY), sum = T(0);
-  for (int i = 0; i < W; ++i) mx = fmax(mx, sm[i]);
-  for (int i = 0; i < W; ++i) sum += sl[i] == T(0) ? T(0) : sl[i] * dev_exp<T>(sm[i] - mx);
+  sum = T(0);
+  for (int i = 0; i < kWarps; ++i) sum += sl[i];
   for (int c = threadIdx.x; c < d; c += kThreads) {
-    T a = T(0);
-    for (int i = 0; i < W; ++i) a += sl[i] == T(0) ? T(0) : sa[i][c] * dev_exp<T>(sm[i] - mx);
-    out[(b * heads + h) * d + c] = n == 0 ? T(0) : a / sum;
+    T v = T(0);
+    for (int i = 0; i < kWarps; ++i) v += sacc[i][c];
+    out[head * d + c] = v / sum;
   }
-  if (threadIdx.x == 0 && lse) lse[b * heads + h] = n == 0 ? T(-INFINITY) : mx + dev_log<T>(sum);
+  if (threadIdx.x == 0 && lse) lse[head] = Base<T>::natural(mx) + dev_log<T>(sum);
+}
+
+int sm_count() {
+  static int n = 0;
+  if (!n) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
+      n = 148;
+  }
+  return n;
+}
+
+// Query heads that one block takes: the group of a key head, rounded up to a power of two, at
+// most 8 (2 where the lanes hold double: more would not fit the registers).
+int heads_per_block(int dtype, int64_t group) {
+  const int most = dtype == TG_F64 ? 2 : 8;
+  int g = 1;
+  while (g < group && g < most) g *= 2;
+  return g;
+}
+
+// Splits of the longest sequence: enough blocks to fill the multiprocessors several times over
+// (sequences end at different lengths), none shorter than kMinSplit.
+int split_count(int dtype, int64_t batch, int64_t heads, int64_t kv_heads, int64_t longest) {
+  const int gh = heads_per_block(dtype, heads / kv_heads);
+  const int64_t groups = (heads / kv_heads + gh - 1) / gh;
+  const int64_t blocks = batch * kv_heads * groups;
+  const int64_t want = (8 * (int64_t)sm_count() + blocks - 1) / blocks;
+  const int64_t most = (longest + kMinSplit - 1) / kMinSplit;
+  const int64_t n = want < most ? want : most;
+  return (int)(n < 1 ? 1 : (n > kMaxSplits ? kMaxSplits : n));
+}
+
+template <typename T, int VE, int LPT, int GH>
+int launch_attend(const AttendArgs& a, int64_t blocks, const T* q, const T* keys, const T* values,
+                  T* out, T* lse, T* part, cudaStream_t s) {
+  using A = Attend<T, VE, LPT, GH>;
+  TG_CUDA_TRY(cudaFuncSetAttribute(paged_attention_kernel<T, VE, LPT, GH>,
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize, A::SMEM));
+  TG_CUDA_TRY(launch_pdl(paged_attention_kernel<T, VE, LPT, GH>, dim3((unsigned)blocks),
+                         dim3(kThreads), A::SMEM, s, a, q, keys, values, out, lse, part));
+  return check_launch("paged_attention");
+}
+
+template <typename T, int VE, int LPT>
+int attend_heads(int gh, const AttendArgs& a, int64_t blocks, const T* q, const T* keys,
+                 const T* values, T* out, T* lse, T* part, cudaStream_t s) {
+  switch (gh) {
+    case 1: return launch_attend<T, VE, LPT, 1>(a, blocks, q, keys, values, out, lse, part, s);
+    case 2: return launch_attend<T, VE, LPT, 2>(a, blocks, q, keys, values, out, lse, part, s);
+  }
+  if constexpr (sizeof(T) == 4) {
+    if (gh == 4)
+      return launch_attend<T, VE, LPT, 4>(a, blocks, q, keys, values, out, lse, part, s);
+    return launch_attend<T, VE, LPT, 8>(a, blocks, q, keys, values, out, lse, part, s);
+  }
+  return set_error(TG_ERR_UNSUPPORTED, "paged_attention: %d heads to a block", gh);
+}
+
+template <typename T, int VE>
+int attend_width(int gh, const AttendArgs& a, int64_t blocks, const T* q, const T* keys,
+                 const T* values, T* out, T* lse, T* part, cudaStream_t s) {
+  const int64_t d = a.pool.head_dim;
+  if (d <= 32) return attend_heads<T, VE, 4>(gh, a, blocks, q, keys, values, out, lse, part, s);
+  if (d <= 64) return attend_heads<T, VE, 8>(gh, a, blocks, q, keys, values, out, lse, part, s);
+  if (d <= 128) return attend_heads<T, VE, 16>(gh, a, blocks, q, keys, values, out, lse, part, s);
+  return attend_heads<T, VE, 32>(gh, a, blocks, q, keys, values, out, lse, part, s);
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -263,7 +607,10 @@ int tg_page_copy(int64_t page_bytes, int64_t layers, int64_t num_pages, void* ke
 
 size_t tg_paged_attention_scratch_bytes(int dtype, int64_t batch, int64_t heads, int64_t kv_heads,
                                         int64_t head_dim, int64_t longest) {
-  return 16;
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || head_dim <= 0) return 16;
+  const int splits = split_count(dtype, batch, heads, kv_heads, longest);
+  if (splits == 1) return 16;
+  return (size_t)(batch * heads * splits * (head_dim + 2)) * (dtype == TG_F64 ? 8 : 4);
 }
 
 int tg_paged_attention(int dtype, int64_t batch, int64_t heads, int64_t kv_heads,
@@ -278,20 +625,42 @@ int tg_paged_attention(int dtype, int64_t batch, int64_t heads, int64_t kv_heads
   TG_CHECK_ARG(batch >= 0 && heads > 0 && heads % kv_heads == 0,
                "paged_attention: %lld query heads over %lld key heads", (long long)heads,
                (long long)kv_heads);
-  TG_CHECK_ARG(batch * heads <= INT32_MAX, "paged_attention: batch too large");
+  TG_CHECK_ARG(num_pages <= INT32_MAX && max_pages <= (INT32_MAX - (1 << 16)) / page_size,
+               "paged_attention: positions up to 2^31 (table of %lld pages of %lld)",
+               (long long)max_pages, (long long)page_size);
   if (head_dim > kMaxHead)
     return set_error(TG_ERR_UNSUPPORTED, "paged_attention: head_dim %lld (at most %d)",
                      (long long)head_dim, kMaxHead);
+  TG_CHECK_ARG(batch <= INT32_MAX / (heads * kMaxSplits), "paged_attention: batch too large");
   if (batch == 0) return TG_OK;
   cudaStream_t s = as_stream(stream);
-  (void)scratch;
-  (void)longest;
   return TG_DISPATCH_FLOAT(dtype, T, [&] {
-    const Pool p{num_pages, kv_heads, page_size, head_dim, pages, max_pages, bad_page_dev};
-    paged_attention_kernel<T><<<(unsigned)(batch * heads), kThreads, 0, s>>>(
-        p, heads, (const T*)q, q_sb, q_sh, (const T*)key_pages, (const T*)value_pages, lengths,
-        (T)(1.0 / sqrt((double)head_dim)), (T*)out, (T*)lse);
-    return check_launch("paged_attention");
+    constexpr int VE = 16 / sizeof(T);
+    AttendArgs a{};
+    a.pool = {num_pages, kv_heads, page_size, head_dim, pages, max_pages, bad_page_dev};
+    a.heads = heads;
+    a.group = heads / kv_heads;
+    const int gh = heads_per_block(dtype, a.group);
+    a.head_groups = (a.group + gh - 1) / gh;
+    a.q_sb = q_sb;
+    a.q_sh = q_sh;
+    a.lengths = lengths;
+    a.splits = split_count(dtype, batch, heads, kv_heads, longest);
+    a.size = make_div(page_size);
+    a.scale = 1.0 / sqrt((double)head_dim);
+    TG_CHECK_ARG(a.splits == 1 || scratch, "paged_attention: no scratch");
+    const int64_t blocks = batch * kv_heads * a.head_groups * a.splits;
+    const int r = head_dim % VE == 0 && aligned16(key_pages) && aligned16(value_pages)
+                      ? attend_width<T, VE>(gh, a, blocks, (const T*)q, (const T*)key_pages,
+                                            (const T*)value_pages, (T*)out, (T*)lse, (T*)scratch,
+                                            s)
+                      : attend_width<T, 1>(gh, a, blocks, (const T*)q, (const T*)key_pages,
+                                           (const T*)value_pages, (T*)out, (T*)lse, (T*)scratch,
+                                           s);
+    if (r || a.splits == 1) return r;
+    TG_CUDA_TRY(launch_pdl(paged_join_kernel<T>, dim3((unsigned)(batch * heads)), dim3(kThreads),
+                           0, s, a, (const T*)scratch, (T*)out, (T*)lse));
+    return check_launch("paged_attention(join)");
   });
 }
 
