@@ -7,6 +7,8 @@
 // Page ids and lengths live on the device and are checked where they are read: an id outside
 // [0, num_pages) reads page 0 or writes nothing, a length beyond the table counts as the
 // table's end, and either sets *bad, which the host reads at its next synchronisation.
+#include <limits>
+
 #include "common.cuh"
 
 namespace tg {
@@ -109,7 +111,7 @@ page_copy_kernel(V* keys, V* values, int64_t layers, int64_t num_pages, int64_t 
 constexpr int kMaxHead = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kLaneDims = 8;        // features of a position that one lane holds
-constexpr int kTable = 2048;        // pages named in shared memory at a time
+constexpr int kTable = 1024;        // pages named in shared memory at a time
 constexpr int kMinSplit = 256;      // positions that a block has at least, if there are as many
 constexpr int kMaxSplits = 512;
 
@@ -164,6 +166,7 @@ struct AttendArgs {
   int64_t heads, group, head_groups;  // query heads; to a key head; blocks that share one
   int64_t q_sb, q_sh;
   const int64_t* lengths;
+  int64_t batch_heads;  // sequences times query heads
   int splits;
   FastDiv size;
   double scale;
@@ -178,22 +181,36 @@ __device__ __forceinline__ int split_length(int n, int splits) {
 }
 
 // One block per (sequence, key head, split of its positions, group of GH query heads). LPT lanes
-// share a position, each with 8 of its features, so a warp has 32 / LPT positions at a time and
-// every lane group runs its own softmax; queries and outputs of GH heads stay in registers. Each
-// lane copies its features of the next ST positions' keys and values into shared memory itself
+// share a position, each with 8 of its features; a lane group takes U positions at a time and runs
+// its own softmax, a warp has 32 / LPT groups, queries and outputs of GH heads stay in registers.
+// Each lane copies its features of the next positions' keys and values into shared memory itself
 // (cp.async, VE elements at a time) and is the only one to read them: no barrier in the loop.
-// What bounds it: reading keys and values once. 2 blocks of 256 lanes keep up to 160 KB a
-// multiprocessor in flight.
+// The U GH scores of a group are reduced by halving: at each of the first levels a lane keeps
+// half of its partial scores and hands the other half over, so that a score is finished, and its
+// exponential taken, in one lane (LPT / (U GH) lanes), and is then dealt out to the group.
+// What bounds it: reading keys and values once; behind that the issue slots (at 4 heads of 128 to
+// a key head they are two thirds taken).
+constexpr int U = 2;
+
+constexpr int log2_of(int x) { return x <= 1 ? 0 : 1 + log2_of(x / 2); }
+
 template <typename T, int VE, int LPT, int GH>
 struct Attend {
   static constexpr int NVEC = kLaneDims / VE;
   static constexpr int VB = VE * (int)sizeof(T);
-  static constexpr int STAGE = 2 * NVEC * VB * kThreads;
-  static constexpr int ST = sizeof(T) == 4 ? 6 : 3;
+  static constexpr int ROW = 2 * NVEC * VB * kThreads;  // one position per lane group
+  static constexpr int STAGE = U * ROW;
+  static constexpr int ST = sizeof(T) == 4 ? 3 : 2;
   static constexpr int WIDTH = LPT * kLaneDims;  // features covered
   static constexpr int RING = ST * STAGE;
   static constexpr int JOIN = kWarps * GH * (WIDTH + 2) * (int)sizeof(T);
-  static constexpr int SMEM = (RING > JOIN ? RING : JOIN) + kTable * 4;
+  static constexpr int SMEM = (RING > JOIN ? RING : JOIN) + kTable * 8;
+  // The scores of a group: value v = u GH + g ends in the lane of the group whose top LEVELS bits
+  // are v's top bits, as its (v % KEPT)-th.
+  static constexpr int V = U * GH;
+  static constexpr int LEVELS = log2_of(LPT) < log2_of(V) ? log2_of(LPT) : log2_of(V);
+  static constexpr int KEPT = V >> LEVELS;
+  static constexpr int lane_of(int v) { return (v / KEPT) << (log2_of(LPT) - LEVELS); }
 };
 
 template <typename T, int VE, int LPT, int GH>
@@ -202,9 +219,11 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
                        const T* __restrict__ values, T* __restrict__ out, T* __restrict__ lse,
                        T* __restrict__ part) {
   using A = Attend<T, VE, LPT, GH>;
-  constexpr int NVEC = A::NVEC, ST = A::ST, TPW = 32 / LPT, STEP = kWarps * TPW;
+  constexpr int NVEC = A::NVEC, ST = A::ST, TPW = 32 / LPT, ROWS = kWarps * TPW, STEP = U * ROWS;
+  constexpr int V = A::V, KEPT = A::KEPT;
+  constexpr T kLowest = std::numeric_limits<T>::lowest();
   extern __shared__ __align__(16) uint8_t smem[];
-  int* table = reinterpret_cast<int*>(smem + A::SMEM - kTable * 4);
+  int64_t* table = reinterpret_cast<int64_t*>(smem + A::SMEM - kTable * 8);
   pdl_trigger();
   pdl_wait();
   int64_t e = blockIdx.x;
@@ -223,11 +242,12 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
   const int64_t h0 = kh * a.group + g0;
   const int live_heads = (int)(a.group - g0 < GH ? a.group - g0 : GH);
 
-  T qr[GH][kLaneDims], acc[GH][kLaneDims], m[GH], l[GH];
+  // m and l belong to the KEPT scores that this lane finishes: the running maximum of that
+  // score's head (the same in every lane of the group that has the head) and the sum over the
+  // positions that came to this lane.
+  T qr[GH][kLaneDims], acc[GH][kLaneDims], m[KEPT], l[KEPT];
 #pragma unroll
-  for (int g = 0; g < GH; ++g) {
-    m[g] = T(-INFINITY);
-    l[g] = T(0);
+  for (int g = 0; g < GH; ++g)
 #pragma unroll
     for (int i = 0; i < kLaneDims; ++i) {
       const int c = ((i / VE) * LPT + j) * VE + i % VE;
@@ -236,20 +256,23 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
                      : T(0);
       acc[g][i] = T(0);
     }
+#pragma unroll
+  for (int r = 0; r < KEPT; ++r) {
+    m[r] = kLowest;
+    l[r] = T(0);
   }
-  const uint32_t ring =
-      (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * A::VB;
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * A::VB;
   const uint8_t* mine = smem + threadIdx.x * A::VB;
   // Features behind the head's width are never copied: they stay zero.
-  for (int i = 0; i < ST * 2 * NVEC; ++i) {
+  for (int i = 0; i < ST * U * 2 * NVEC; ++i) {
     if (((i % NVEC) * LPT + j) * VE < d) continue;
     T* z = reinterpret_cast<T*>(smem + threadIdx.x * A::VB + i * (A::VB * kThreads));
 #pragma unroll
     for (int v = 0; v < VE; ++v) z[v] = T(0);
   }
-  const int64_t page_rows = a.pool.kv_heads * a.pool.page_size;
+  const int my_row = w * TPW + sub;  // of the ROWS positions of a round
   for (int t0 = begin; t0 < end;) {
-    // The pages of the next positions, as many as the table holds.
+    // Where the pages of the next positions start, as many as the table holds.
     const int p0 = div_by(t0, a.size);
     const int64_t stop = (int64_t)(p0 + kTable) * a.size.d;
     const int t1 = stop < end ? (int)stop : end;
@@ -261,87 +284,146 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
         if (a.pool.bad) *a.pool.bad = 1;
         page = 0;
       }
-      table[i] = (int)page;
+      table[i] = (page * a.pool.kv_heads + kh) * a.pool.page_size * d;
     }
     __syncthreads();
     const int steps = (t1 - t0 + STEP - 1) / STEP;
     auto issue = [&](int i) {
-      const int t = t0 + i * STEP + w * TPW + sub;
-      const bool live = i < steps && t < t1;
-      int64_t at = 0;
-      if (live) {
-        const int p = div_by(t, a.size);
-        at = (table[p - p0] * page_rows + kh * a.pool.page_size + (t - p * (int)a.size.d)) * d;
-      }
-      const uint32_t to = ring + (i % ST) * A::STAGE;
 #pragma unroll
-      for (int v = 0; v < NVEC; ++v) {
-        const int c = (v * LPT + j) * VE;
-        if (c < d) {
-          copy_async<A::VB>(to + v * (A::VB * kThreads), keys + at + c, live);
-          copy_async<A::VB>(to + (NVEC + v) * (A::VB * kThreads), values + at + c, live);
+      for (int u = 0; u < U; ++u) {
+        const int t = t0 + i * STEP + u * ROWS + my_row;
+        const bool live = t < t1;
+        int64_t at = j * VE;
+        if (live) {
+          const int p = div_by(t, a.size);
+          at += table[p - p0] + (int64_t)(t - p * (int)a.size.d) * d;
         }
+        const uint32_t to = ring + (i % ST) * A::STAGE + u * A::ROW;
+        const T* k = keys + at;
+        const T* v = values + at;
+#pragma unroll
+        for (int x = 0; x < NVEC; ++x)
+          if ((x * LPT + j) * VE < d) {
+            copy_async<A::VB>(to + x * (A::VB * kThreads), k + x * (LPT * VE), live);
+            copy_async<A::VB>(to + (NVEC + x) * (A::VB * kThreads), v + x * (LPT * VE), live);
+          }
       }
-      copy_commit();
     };
 #pragma unroll
-    for (int i = 0; i < ST - 1; ++i) issue(i);
+    for (int i = 0; i < ST - 1; ++i) {
+      if (i < steps) issue(i);
+      copy_commit();
+    }
     for (int i = 0; i < steps; ++i) {
       copy_wait<ST - 2>();
       const uint8_t* from = mine + (i % ST) * A::STAGE;
-      T x[kLaneDims], s[GH];
+      auto load = [&](T (&x)[kLaneDims], const uint8_t* row) {
 #pragma unroll
-      for (int v = 0; v < NVEC; ++v)
+        for (int v = 0; v < NVEC; ++v)
 #pragma unroll
-        for (int u = 0; u < VE; ++u)
-          x[v * VE + u] = reinterpret_cast<const T*>(from + v * (A::VB * kThreads))[u];
+          for (int c = 0; c < VE; ++c)
+            x[v * VE + c] = reinterpret_cast<const T*>(row + v * (A::VB * kThreads))[c];
+      };
+      T s[V];
 #pragma unroll
-      for (int g = 0; g < GH; ++g) {
-        s[g] = T(0);
+      for (int u = 0; u < U; ++u) {
+        T x[kLaneDims];
+        load(x, from + u * A::ROW);
 #pragma unroll
-        for (int c = 0; c < kLaneDims; ++c) s[g] += qr[g][c] * x[c];
-      }
+        for (int g = 0; g < GH; ++g) {
+          T dot = T(0);
 #pragma unroll
-      for (int o = LPT / 2; o > 0; o >>= 1)
-#pragma unroll
-        for (int g = 0; g < GH; ++g) s[g] += __shfl_xor_sync(0xffffffffu, s[g], o);
-#pragma unroll
-      for (int v = 0; v < NVEC; ++v)
-#pragma unroll
-        for (int u = 0; u < VE; ++u)
-          x[v * VE + u] = reinterpret_cast<const T*>(from + (NVEC + v) * (A::VB * kThreads))[u];
-      const bool live = t0 + i * STEP + w * TPW + sub < t1;
-#pragma unroll
-      for (int g = 0; g < GH; ++g) {
-        if (!live || s[g] == T(-INFINITY)) continue;
-        if (s[g] > m[g]) {
-          const T c = Base<T>::exp_(m[g] - s[g]);
-          m[g] = s[g];
-          l[g] *= c;
-#pragma unroll
-          for (int k = 0; k < kLaneDims; ++k) acc[g][k] *= c;
+          for (int c = 0; c < kLaneDims; ++c) dot += qr[g][c] * x[c];
+          s[u * GH + g] = dot;
         }
-        const T p = Base<T>::exp_(s[g] - m[g]);
-        l[g] += p;
-#pragma unroll
-        for (int k = 0; k < kLaneDims; ++k) acc[g][k] += p * x[k];
       }
-      issue(i + ST - 1);
+#pragma unroll
+      for (int k = 0; k < log2_of(LPT); ++k) {
+        const int o = LPT >> (k + 1);
+        if (k < A::LEVELS) {
+          const int half = V >> (k + 1);
+          const bool upper = j & o;
+#pragma unroll
+          for (int v = 0; v < half; ++v) {
+            const T give = upper ? s[v] : s[v + half], keep = upper ? s[v + half] : s[v];
+            s[v] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+          }
+        } else {
+#pragma unroll
+          for (int v = 0; v < KEPT; ++v) s[v] += __shfl_xor_sync(0xffffffffu, s[v], o);
+        }
+      }
+      // s[0..KEPT): this lane's finished scores; its position is the first or second of the
+      // group's two by its top bit.
+      const int left = t1 - (t0 + i * STEP + my_row);
+      const bool live = left > (j & (LPT / 2) ? ROWS : 0);
+      bool grows = false;
+#pragma unroll
+      for (int r = 0; r < KEPT; ++r) {
+        if (!live) s[r] = T(-INFINITY);
+        grows |= s[r] > m[r];
+      }
+      if (__any_sync(0xffffffffu, grows)) {
+        T c[KEPT];
+#pragma unroll
+        for (int r = 0; r < KEPT; ++r) {
+          const T other = __shfl_xor_sync(0xffffffffu, s[r], LPT / 2);
+          const T top = fmax(m[r], fmax(s[r], other));
+          c[r] = Base<T>::exp_(m[r] - top);
+          m[r] = top;
+          l[r] *= c[r];
+        }
+#pragma unroll
+        for (int g = 0; g < GH; ++g) {
+          const T cg = __shfl_sync(0xffffffffu, c[g % KEPT], sub * LPT + A::lane_of(g));
+#pragma unroll
+          for (int k = 0; k < kLaneDims; ++k) acc[g][k] *= cg;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < KEPT; ++r) {
+        s[r] = Base<T>::exp_(s[r] - m[r]);
+        l[r] += s[r];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        T x[kLaneDims];
+        load(x, from + u * A::ROW + NVEC * (A::VB * kThreads));
+#pragma unroll
+        for (int g = 0; g < GH; ++g) {
+          const int v = u * GH + g;
+          const T p = __shfl_sync(0xffffffffu, s[v % KEPT], sub * LPT + A::lane_of(v));
+#pragma unroll
+          for (int k = 0; k < kLaneDims; ++k) acc[g][k] += p * x[k];
+        }
+      }
+      if (i + ST - 1 < steps) issue(i + ST - 1);
+      copy_commit();
     }
     copy_wait<0>();
     t0 = t1;
   }
 
-  // The warp's lane groups, then the block's warps.
+  // Every lane learns its heads' maxima and sums, then the warp's lane groups join, then the
+  // block's warps.
+  T mg[GH], lg[GH];
+#pragma unroll
+  for (int g = 0; g < GH; ++g) {
+    mg[g] = __shfl_sync(0xffffffffu, m[g % KEPT], sub * LPT + A::lane_of(g));
+    lg[g] = T(0);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      lg[g] += __shfl_sync(0xffffffffu, l[g % KEPT], sub * LPT + A::lane_of(u * GH + g));
+  }
 #pragma unroll
   for (int o = LPT; o < 32; o <<= 1)
 #pragma unroll
     for (int g = 0; g < GH; ++g) {
-      const T om = __shfl_xor_sync(0xffffffffu, m[g], o), mx = fmax(m[g], om);
-      const T c = l[g] == T(0) ? T(0) : Base<T>::exp_(m[g] - mx);
-      l[g] *= c;
-      l[g] += __shfl_xor_sync(0xffffffffu, l[g], o);
-      m[g] = mx;
+      const T top = fmax(mg[g], __shfl_xor_sync(0xffffffffu, mg[g], o));
+      const T c = lg[g] == T(0) ? T(0) : Base<T>::exp_(mg[g] - top);
+      lg[g] *= c;
+      lg[g] += __shfl_xor_sync(0xffffffffu, lg[g], o);
+      mg[g] = top;
 #pragma unroll
       for (int k = 0; k < kLaneDims; ++k) {
         acc[g][k] *= c;
@@ -359,8 +441,8 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
       for (int k = 0; k < kLaneDims; ++k)
         sacc[(w * GH + g) * A::WIDTH + ((k / VE) * LPT + j) * VE + k % VE] = acc[g][k];
       if (j == 0) {
-        sm[w * GH + g] = m[g];
-        sl[w * GH + g] = l[g];
+        sm[w * GH + g] = mg[g];
+        sl[w * GH + g] = lg[g];
       }
     }
   }
@@ -368,13 +450,13 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
   const bool whole = n <= len;  // no other split of this sequence
   for (int i = threadIdx.x; i < live_heads * d; i += kThreads) {
     const int g = i / d, c = i % d;
-    T mx = T(-INFINITY), sum = T(0), v = T(0);
+    T top = kLowest, sum = T(0), v = T(0);
 #pragma unroll
-    for (int k = 0; k < kWarps; ++k) mx = fmax(mx, sm[k * GH + g]);
+    for (int k = 0; k < kWarps; ++k) top = fmax(top, sm[k * GH + g]);
 #pragma unroll
     for (int k = 0; k < kWarps; ++k) {
       const T ls = sl[k * GH + g];
-      const T f = ls == T(0) ? T(0) : Base<T>::exp_(sm[k * GH + g] - mx);
+      const T f = ls == T(0) ? T(0) : Base<T>::exp_(sm[k * GH + g] - top);
       sum += ls * f;
       v += (ls == T(0) ? T(0) : sacc[(k * GH + g) * A::WIDTH + c]) * f;
     }
@@ -382,26 +464,25 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
     if (whole) {
       out[head * d + c] = n == 0 ? T(0) : v / sum;
       if (c == 0 && lse)
-        lse[head] = n == 0 ? T(-INFINITY) : Base<T>::natural(mx) + dev_log<T>(sum);
+        lse[head] = n == 0 ? T(-INFINITY) : Base<T>::natural(top) + dev_log<T>(sum);
     } else {
-      T* to = part + (head * a.splits + split) * (d + 2);
-      to[2 + c] = v;
+      T* ml = part + (head * a.splits + split) * 2;
+      part[a.batch_heads * a.splits * 2 + (head * a.splits + split) * d + c] = v;
       if (c == 0) {
-        to[0] = mx;
-        to[1] = sum;
+        ml[0] = top;
+        ml[1] = sum;
       }
     }
   }
 }
 
-// The splits of a sequence's head as one: block per (sequence, head), the splits dealt to the
-// warps.
+// The splits of a sequence's head as one: block per (sequence, head), their weights found once,
+// their outputs dealt to the warps.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 paged_join_kernel(AttendArgs a, const T* __restrict__ part, T* __restrict__ out,
                   T* __restrict__ lse) {
-  constexpr int N = kMaxHead / 32;
-  __shared__ T sacc[kWarps][kMaxHead], sl[kWarps];
+  __shared__ T weight[kMaxSplits], red[32], sacc[kWarps][kMaxHead];
   pdl_wait();
   const int64_t head = blockIdx.x, b = head / a.heads;
   const int d = (int)a.pool.head_dim, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -409,31 +490,31 @@ paged_join_kernel(AttendArgs a, const T* __restrict__ part, T* __restrict__ out,
   const int len = split_length(n, a.splits);
   if (n <= len) return;  // written by its only block
   const int live = (n + len - 1) / len;
-  const T* from = part + head * a.splits * (d + 2);
-  T mx = T(-INFINITY);
-  for (int i = lane; i < live; i += 32) mx = fmax(mx, from[(int64_t)i * (d + 2)]);
-  mx = warp_max(mx);
-  T acc[N] = {}, sum = T(0);
-  for (int i = w; i < live; i += kWarps) {
-    const T* p = from + (int64_t)i * (d + 2);
-    const T ls = p[1], f = ls == T(0) ? T(0) : Base<T>::exp_(p[0] - mx);
+  const T* ml = part + head * a.splits * 2;
+  T top = std::numeric_limits<T>::lowest(), sum = T(0);
+  for (int i = threadIdx.x; i < live; i += kThreads) top = fmax(top, ml[2 * i]);
+  top = block_max(top, red);
+  for (int i = threadIdx.x; i < live; i += kThreads) {
+    const T ls = ml[2 * i + 1], f = ls == T(0) ? T(0) : Base<T>::exp_(ml[2 * i] - top);
+    weight[i] = f;
     sum += ls * f;
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-      if (lane + 32 * k < d) acc[k] += p[2 + lane + 32 * k] * f;
   }
-  if (lane == 0) sl[w] = sum;
-#pragma unroll
-  for (int k = 0; k < N; ++k) sacc[w][lane + 32 * k] = acc[k];
+  sum = block_sum(sum, red);  // its barriers also publish the weights
+  const T* from = part + a.batch_heads * a.splits * 2 + head * a.splits * d;
+  for (int c = lane; c < d; c += 32) {
+    T v = T(0);
+#pragma unroll 4
+    for (int i = w; i < live; i += kWarps) v += from[(int64_t)i * d + c] * weight[i];
+    sacc[w][c] = v;
+  }
   __syncthreads();
-  sum = T(0);
-  for (int i = 0; i < kWarps; ++i) sum += sl[i];
   for (int c = threadIdx.x; c < d; c += kThreads) {
     T v = T(0);
+#pragma unroll
     for (int i = 0; i < kWarps; ++i) v += sacc[i][c];
     out[head * d + c] = v / sum;
   }
-  if (threadIdx.x == 0 && lse) lse[head] = Base<T>::natural(mx) + dev_log<T>(sum);
+  if (threadIdx.x == 0 && lse) lse[head] = Base<T>::natural(top) + dev_log<T>(sum);
 }
 
 int sm_count() {
@@ -642,6 +723,7 @@ int tg_paged_attention(int dtype, int64_t batch, int64_t heads, int64_t kv_heads
     a.group = heads / kv_heads;
     const int gh = heads_per_block(dtype, a.group);
     a.head_groups = (a.group + gh - 1) / gh;
+    a.batch_heads = batch * heads;
     a.q_sb = q_sb;
     a.q_sh = q_sh;
     a.lengths = lengths;
