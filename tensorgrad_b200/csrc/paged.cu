@@ -7,6 +7,8 @@
 // Page ids and lengths live on the device and are checked where they are read: an id outside
 // [0, num_pages) reads page 0 or writes nothing, a length beyond the table counts as the
 // table's end, and either sets *bad, which the host reads at its next synchronisation.
+#include <cooperative_groups.h>
+
 #include <limits>
 
 #include "common.cuh"
@@ -109,11 +111,13 @@ page_copy_kernel(V* keys, V* values, int64_t layers, int64_t num_pages, int64_t 
 
 // ---------------------------------------------------------------- attention of one token
 constexpr int kMaxHead = 256;
-constexpr int kWarps = kThreads / 32;
+constexpr int kAttend = 128;        // threads of an attention block
+constexpr int kWarps = kAttend / 32;
 constexpr int kLaneDims = 8;        // features of a position that one lane holds
-constexpr int kTable = 1024;        // pages named in shared memory at a time
-constexpr int kMinSplit = 256;      // positions that a block has at least, if there are as many
+constexpr int kTable = 512;        // pages named in shared memory at a time
+constexpr int kMinSplit = 128;      // positions that a block has at least, if there are as many
 constexpr int kMaxSplits = 512;
+constexpr int kMaxCluster = 8;      // splits that join through their cluster's shared memory
 
 // n / d for 0 <= n < 2^31 by a multiplication (d fixed for a launch; Granlund and Montgomery,
 // "Division by invariant integers using multiplication", 1994).
@@ -168,6 +172,7 @@ struct AttendArgs {
   const int64_t* lengths;
   int64_t batch_heads;  // sequences times query heads
   int splits;
+  bool clustered;       // a sequence's splits are one cluster
   FastDiv size;
   double scale;
 };
@@ -198,12 +203,13 @@ template <typename T, int VE, int LPT, int GH>
 struct Attend {
   static constexpr int NVEC = kLaneDims / VE;
   static constexpr int VB = VE * (int)sizeof(T);
-  static constexpr int ROW = 2 * NVEC * VB * kThreads;  // one position per lane group
+  static constexpr int ROW = 2 * NVEC * VB * kAttend;  // one position per lane group
   static constexpr int STAGE = U * ROW;
   static constexpr int ST = sizeof(T) == 4 ? 3 : 2;
   static constexpr int WIDTH = LPT * kLaneDims;  // features covered
   static constexpr int RING = ST * STAGE;
-  static constexpr int JOIN = kWarps * GH * (WIDTH + 2) * (int)sizeof(T);
+  // The warps' results and the block's, with a maximum and a sum each.
+  static constexpr int JOIN = (kWarps + 1) * GH * (WIDTH + 2) * (int)sizeof(T);
   static constexpr int SMEM = (RING > JOIN ? RING : JOIN) + kTable * 8;
   // The scores of a group: value v = u GH + g ends in the lane of the group whose top LEVELS bits
   // are v's top bits, as its (v % KEPT)-th.
@@ -214,7 +220,7 @@ struct Attend {
 };
 
 template <typename T, int VE, int LPT, int GH>
-__global__ void __launch_bounds__(kThreads, GH == 8 ? 1 : 2)
+__global__ void __launch_bounds__(kAttend, GH == 8 ? 2 : 4)
 paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restrict__ keys,
                        const T* __restrict__ values, T* __restrict__ out, T* __restrict__ lse,
                        T* __restrict__ part) {
@@ -227,16 +233,16 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
   pdl_trigger();
   pdl_wait();
   int64_t e = blockIdx.x;
-  const int64_t g0 = (e % a.head_groups) * GH;
-  e /= a.head_groups;
   const int split = (int)(e % a.splits);
   e /= a.splits;
+  const int64_t g0 = (e % a.head_groups) * GH;
+  e /= a.head_groups;
   const int64_t kh = e % a.pool.kv_heads, b = e / a.pool.kv_heads;
   const int d = (int)a.pool.head_dim;
   const int n = (int)length_of(a.pool, a.lengths, b);
   const int len = split_length(n, a.splits);
   const int begin = split * len, end = begin + len < n ? begin + len : n;
-  if (begin >= n && split > 0) return;
+  if (begin >= n && split > 0 && !a.clustered) return;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int sub = lane / LPT, j = lane % LPT;
   const int64_t h0 = kh * a.group + g0;
@@ -266,7 +272,7 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
   // Features behind the head's width are never copied: they stay zero.
   for (int i = 0; i < ST * U * 2 * NVEC; ++i) {
     if (((i % NVEC) * LPT + j) * VE < d) continue;
-    T* z = reinterpret_cast<T*>(smem + threadIdx.x * A::VB + i * (A::VB * kThreads));
+    T* z = reinterpret_cast<T*>(smem + threadIdx.x * A::VB + i * (A::VB * kAttend));
 #pragma unroll
     for (int v = 0; v < VE; ++v) z[v] = T(0);
   }
@@ -278,7 +284,7 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
     const int t1 = stop < end ? (int)stop : end;
     const int used = div_by(t1 - 1, a.size) - p0 + 1;
     __syncthreads();
-    for (int i = threadIdx.x; i < used; i += kThreads) {
+    for (int i = threadIdx.x; i < used; i += kAttend) {
       int64_t page = a.pool.table[b * a.pool.max_pages + p0 + i];
       if (page < 0 || page >= a.pool.num_pages) {
         if (a.pool.bad) *a.pool.bad = 1;
@@ -304,8 +310,8 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
 #pragma unroll
         for (int x = 0; x < NVEC; ++x)
           if ((x * LPT + j) * VE < d) {
-            copy_async<A::VB>(to + x * (A::VB * kThreads), k + x * (LPT * VE), live);
-            copy_async<A::VB>(to + (NVEC + x) * (A::VB * kThreads), v + x * (LPT * VE), live);
+            copy_async<A::VB>(to + x * (A::VB * kAttend), k + x * (LPT * VE), live);
+            copy_async<A::VB>(to + (NVEC + x) * (A::VB * kAttend), v + x * (LPT * VE), live);
           }
       }
     };
@@ -322,7 +328,7 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
         for (int v = 0; v < NVEC; ++v)
 #pragma unroll
           for (int c = 0; c < VE; ++c)
-            x[v * VE + c] = reinterpret_cast<const T*>(row + v * (A::VB * kThreads))[c];
+            x[v * VE + c] = reinterpret_cast<const T*>(row + v * (A::VB * kAttend))[c];
       };
       T s[V];
 #pragma unroll
@@ -388,7 +394,7 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         T x[kLaneDims];
-        load(x, from + u * A::ROW + NVEC * (A::VB * kThreads));
+        load(x, from + u * A::ROW + NVEC * (A::VB * kAttend));
 #pragma unroll
         for (int g = 0; g < GH; ++g) {
           const int v = u * GH + g;
@@ -448,7 +454,10 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
   }
   __syncthreads();
   const bool whole = n <= len;  // no other split of this sequence
-  for (int i = threadIdx.x; i < live_heads * d; i += kThreads) {
+  T* rt = sl + kWarps * GH;     // [GH], the block's maxima, sums and outputs
+  T* rs = rt + GH;
+  T* rv = rs + GH;
+  for (int i = threadIdx.x; i < live_heads * d; i += kAttend) {
     const int g = i / d, c = i % d;
     T top = kLowest, sum = T(0), v = T(0);
 #pragma unroll
@@ -461,7 +470,13 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
       v += (ls == T(0) ? T(0) : sacc[(k * GH + g) * A::WIDTH + c]) * f;
     }
     const int64_t head = b * a.heads + h0 + g;
-    if (whole) {
+    if (a.clustered) {
+      rv[g * d + c] = v;
+      if (c == 0) {
+        rt[g] = top;
+        rs[g] = sum;
+      }
+    } else if (whole) {
       out[head * d + c] = n == 0 ? T(0) : v / sum;
       if (c == 0 && lse)
         lse[head] = n == 0 ? T(-INFINITY) : Base<T>::natural(top) + dev_log<T>(sum);
@@ -474,15 +489,37 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
       }
     }
   }
+  if (!a.clustered) return;
+  // The splits of this sequence are this cluster's blocks: each joins a share of the outputs.
+  const auto cluster = cooperative_groups::this_cluster();
+  cluster.sync();
+  for (int i = split * kAttend + threadIdx.x; i < live_heads * d; i += a.splits * kAttend) {
+    const int g = i / d, c = i % d;
+    T top = kLowest, sum = T(0), v = T(0);
+    for (int r = 0; r < a.splits; ++r) top = fmax(top, cluster.map_shared_rank(rt, r)[g]);
+    for (int r = 0; r < a.splits; ++r) {
+      const T ls = cluster.map_shared_rank(rs, r)[g];
+      const T f = ls == T(0) ? T(0) : Base<T>::exp_(cluster.map_shared_rank(rt, r)[g] - top);
+      sum += ls * f;
+      v += (ls == T(0) ? T(0) : cluster.map_shared_rank(rv, r)[i]) * f;
+    }
+    const int64_t head = b * a.heads + h0 + g;
+    out[head * d + c] = n == 0 ? T(0) : v / sum;
+    if (c == 0 && lse)
+      lse[head] = n == 0 ? T(-INFINITY) : Base<T>::natural(top) + dev_log<T>(sum);
+  }
+  cluster.sync();  // the others may still read this block's results
 }
 
 // The splits of a sequence's head as one: block per (sequence, head), their weights found once,
 // their outputs dealt to the warps.
+constexpr int kJoinWarps = kThreads / 32;
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 paged_join_kernel(AttendArgs a, const T* __restrict__ part, T* __restrict__ out,
                   T* __restrict__ lse) {
-  __shared__ T weight[kMaxSplits], red[32], sacc[kWarps][kMaxHead];
+  __shared__ T weight[kMaxSplits], red[32], sacc[kJoinWarps][kMaxHead];
   pdl_wait();
   const int64_t head = blockIdx.x, b = head / a.heads;
   const int d = (int)a.pool.head_dim, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -504,14 +541,14 @@ paged_join_kernel(AttendArgs a, const T* __restrict__ part, T* __restrict__ out,
   for (int c = lane; c < d; c += 32) {
     T v = T(0);
 #pragma unroll 4
-    for (int i = w; i < live; i += kWarps) v += from[(int64_t)i * d + c] * weight[i];
+    for (int i = w; i < live; i += kJoinWarps) v += from[(int64_t)i * d + c] * weight[i];
     sacc[w][c] = v;
   }
   __syncthreads();
   for (int c = threadIdx.x; c < d; c += kThreads) {
     T v = T(0);
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) v += sacc[i][c];
+    for (int i = 0; i < kJoinWarps; ++i) v += sacc[i][c];
     out[head * d + c] = v / sum;
   }
   if (threadIdx.x == 0 && lse) lse[head] = Base<T>::natural(top) + dev_log<T>(sum);
@@ -537,16 +574,23 @@ int heads_per_block(int dtype, int64_t group) {
   return g;
 }
 
-// Splits of the longest sequence: enough blocks to fill the multiprocessors several times over
-// (sequences end at different lengths), none shorter than kMinSplit.
+// Splits of the longest sequence: none where the sequences and heads alone give every
+// multiprocessor its 4 blocks (768 of them, up to 1024 positions of 64: 45.5 us unsplit, 47.0 in
+// halves), else about twice that many blocks (32 of them, up to 65536 positions of 128: 252, 236
+// and 250 us with 1, 2 and 3 times), none shorter than kMinSplit (one sequence of 1024 positions
+// on 12 heads: 8.4, 7.1 and 8.4 us with 64, 128 and 256).
 int split_count(int dtype, int64_t batch, int64_t heads, int64_t kv_heads, int64_t longest) {
   const int gh = heads_per_block(dtype, heads / kv_heads);
   const int64_t groups = (heads / kv_heads + gh - 1) / gh;
-  const int64_t blocks = batch * kv_heads * groups;
-  const int64_t want = (8 * (int64_t)sm_count() + blocks - 1) / blocks;
+  const int64_t blocks = batch * kv_heads * groups, slots = 4 * (int64_t)sm_count();
+  if (blocks >= slots) return 1;
+  const int64_t want = (2 * slots + blocks - 1) / blocks;
   const int64_t most = (longest + kMinSplit - 1) / kMinSplit;
   const int64_t n = want < most ? want : most;
-  return (int)(n < 1 ? 1 : (n > kMaxSplits ? kMaxSplits : n));
+  if (n > kMaxCluster) return (int)(n > kMaxSplits ? kMaxSplits : n);
+  int c = 1;  // clusters of 1, 2, 4 and 8
+  while (c < n) c *= 2;
+  return c;
 }
 
 template <typename T, int VE, int LPT, int GH>
@@ -555,8 +599,20 @@ int launch_attend(const AttendArgs& a, int64_t blocks, const T* q, const T* keys
   using A = Attend<T, VE, LPT, GH>;
   TG_CUDA_TRY(cudaFuncSetAttribute(paged_attention_kernel<T, VE, LPT, GH>,
                                    cudaFuncAttributeMaxDynamicSharedMemorySize, A::SMEM));
-  TG_CUDA_TRY(launch_pdl(paged_attention_kernel<T, VE, LPT, GH>, dim3((unsigned)blocks),
-                         dim3(kThreads), A::SMEM, s, a, q, keys, values, out, lse, part));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(kAttend);
+  cfg.dynamicSmemBytes = A::SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim = {(unsigned)(a.clustered ? a.splits : 1), 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  TG_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_attention_kernel<T, VE, LPT, GH>, a, q, keys, values,
+                                 out, lse, part));
   return check_launch("paged_attention");
 }
 
@@ -690,7 +746,7 @@ size_t tg_paged_attention_scratch_bytes(int dtype, int64_t batch, int64_t heads,
                                         int64_t head_dim, int64_t longest) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || head_dim <= 0) return 16;
   const int splits = split_count(dtype, batch, heads, kv_heads, longest);
-  if (splits == 1) return 16;
+  if (splits <= kMaxCluster) return 16;
   return (size_t)(batch * heads * splits * (head_dim + 2)) * (dtype == TG_F64 ? 8 : 4);
 }
 
@@ -728,9 +784,11 @@ int tg_paged_attention(int dtype, int64_t batch, int64_t heads, int64_t kv_heads
     a.q_sh = q_sh;
     a.lengths = lengths;
     a.splits = split_count(dtype, batch, heads, kv_heads, longest);
+    a.clustered = a.splits > 1 && a.splits <= kMaxCluster;
     a.size = make_div(page_size);
     a.scale = 1.0 / sqrt((double)head_dim);
-    TG_CHECK_ARG(a.splits == 1 || scratch, "paged_attention: no scratch");
+    const bool joins = a.splits > kMaxCluster;
+    TG_CHECK_ARG(!joins || scratch, "paged_attention: no scratch");
     const int64_t blocks = batch * kv_heads * a.head_groups * a.splits;
     const int r = head_dim % VE == 0 && aligned16(key_pages) && aligned16(value_pages)
                       ? attend_width<T, VE>(gh, a, blocks, (const T*)q, (const T*)key_pages,
@@ -739,7 +797,7 @@ int tg_paged_attention(int dtype, int64_t batch, int64_t heads, int64_t kv_heads
                       : attend_width<T, 1>(gh, a, blocks, (const T*)q, (const T*)key_pages,
                                            (const T*)value_pages, (T*)out, (T*)lse, (T*)scratch,
                                            s);
-    if (r || a.splits == 1) return r;
+    if (r || !joins) return r;
     TG_CUDA_TRY(launch_pdl(paged_join_kernel<T>, dim3((unsigned)(batch * heads)), dim3(kThreads),
                            0, s, a, (const T*)scratch, (T*)out, (T*)lse));
     return check_launch("paged_attention(join)");
