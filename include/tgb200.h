@@ -115,6 +115,8 @@ uint64_t tg_gemm_fallback_count(void);
 int tg_gemm_tc_status(int reset);
 /* The same record for the fused attention kernels (forward; P and dS of the backward). */
 int tg_attention_tc_status(int reset);
+/* And for the 8-bit integer products (tg_int8_linear). */
+int tg_int8_tc_status(int reset);
 /* Test support for those bounded waits (no reference counterpart): budget_cycles sets the
  * cycle budget of every wait in the fused attention kernels (<= 0 restores the default,
  * about two seconds); withhold_loads != 0 makes the forward's producer issue no load, so its

@@ -7,6 +7,12 @@
 #include "common.cuh"
 
 namespace tg {
+
+// The product on the tensor cores (int8_tc.cu): q (rows, padded inner), float scales and outputs.
+int int8_gemm_tc(const int8_t* q, const int8_t* weight, int64_t ld, const float* row_scales,
+                 const float* scales, const float* bias, float* y, int64_t rows, int64_t inner,
+                 int64_t outer, cudaStream_t stream);
+
 namespace {
 
 constexpr int kThreads = 256;
@@ -22,12 +28,35 @@ __device__ __forceinline__ int quantize(T x, T scale) {
   return (int)fmin(fmax(r, T(-127)), T(127));
 }
 
+// The same by the scale's reciprocal: x * (1 / scale) is off the quotient by less than 2^-15 (two
+// roundings at a size of at most 127 in float), so wherever it is not within 2^-13 of a half both
+// have the same nearest integer; there, and for scales whose reciprocal may overflow, the
+// division decides. 8192 x 4096 values: 59 us with a division each, 31 us with the reciprocal.
+template <typename T>
+struct Reciprocal {
+  T scale, inv;
+  __device__ explicit Reciprocal(T s) : scale(s), inv(s > T(1e-30) ? T(1) / s : T(NAN)) {}
+  __device__ __forceinline__ int of(T x) const {
+    const T q = x * inv, r = rint(q);
+    if (fabs(fabs(q - r) - T(0.5)) > T(0.0001220703125)) return (int)r;
+    return quantize(x, scale);  // also where inv is NaN: no comparison holds
+  }
+};
+
+// A row's scale from its largest magnitude; `odd` is NaN if the row has a NaN or an infinity.
+template <typename T>
+__device__ __forceinline__ T scale_of(T top, T odd) {
+  return top / T(127) + odd;
+}
+
 // Row scales and integers; integer rows are ld bytes long, zero beyond the row's values.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 quantize_rows_kernel(const T* __restrict__ x, int64_t rows, int64_t inner, int8_t* __restrict__ q,
                      int64_t ld, T* __restrict__ scales) {
   __shared__ T sh[32];
+  pdl_trigger();
+  pdl_wait();
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* a = x + r * inner;
     T top = T(0), odd = T(0);
@@ -38,12 +67,152 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t rows, int64_t inner, int8_
     }
     top = block_max(top, sh);
     odd = block_sum(odd, sh);
-    const T scale = top / T(127) + odd;
+    const T scale = scale_of(top, odd);
     const bool live = scale > T(0);
+    const Reciprocal<T> by(scale);
     for (int64_t c = threadIdx.x; c < ld; c += kThreads)
-      q[r * ld + c] = (int8_t)(live && c < inner ? quantize(a[c], scale) : 0);
+      q[r * ld + c] = (int8_t)(live && c < inner ? by.of(a[c]) : 0);
     if (threadIdx.x == 0) scales[r] = scale;
     __syncthreads();
+  }
+}
+
+// Float rows of 16-byte groups, at most N of them to a thread: one read of the row, which stays
+// in registers between its maximum and its integers. HBM-bound: 5 bytes a value.
+template <int N>
+__global__ void __launch_bounds__(kThreads)
+quantize_rows_vec4_kernel(const float4* __restrict__ x, int64_t rows, int groups,
+                          char4* __restrict__ q, int64_t ld4, float* __restrict__ scales) {
+  __shared__ float sh[2][kThreads / 32];
+  pdl_trigger();
+  pdl_wait();
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    float4 v[N];
+    float top = 0.f, odd = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = threadIdx.x + i * kThreads;
+      v[i] = c < groups ? x[r * groups + c] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      top = fmaxf(top, fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
+      odd += (v[i].x - v[i].x) + (v[i].y - v[i].y) + (v[i].z - v[i].z) + (v[i].w - v[i].w);
+    }
+    top = warp_max(top);
+    odd = warp_sum(odd);
+    __syncthreads();  // the last row's readers are done
+    if ((threadIdx.x & 31) == 0) {
+      sh[0][threadIdx.x >> 5] = top;
+      sh[1][threadIdx.x >> 5] = odd;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) {
+      top = fmaxf(top, sh[0][i]);
+      odd += sh[1][i];
+    }
+    const float scale = scale_of(top, odd);
+    const bool live = scale > 0.f;
+    const Reciprocal<float> by(scale);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = threadIdx.x + i * kThreads;
+      if (c >= ld4) continue;
+      char4 o = make_char4(0, 0, 0, 0);
+      if (live)
+        o = make_char4((signed char)by.of(v[i].x), (signed char)by.of(v[i].y),
+                       (signed char)by.of(v[i].z), (signed char)by.of(v[i].w));
+      q[r * ld4 + c] = o;
+    }
+    if (threadIdx.x == 0) scales[r] = scale;
+  }
+}
+
+// Up to R rows of input: every block quantises them into shared memory itself, then its warps
+// walk the output channels, CH at a time, 16 bytes of a weight row to a lane. One launch; what
+// bounds it is reading the weights once, and for small layers the launch.
+template <typename T, int R, int CH>
+__global__ void __launch_bounds__(kThreads)
+few_rows_kernel(const T* __restrict__ x, int rows, int inner, const int8_t* __restrict__ weight,
+                int64_t ld, const T* __restrict__ scales, const T* __restrict__ bias,
+                T* __restrict__ y, int64_t outer) {
+  constexpr int W = kThreads / 32, PER = W / R;  // warps to a row
+  extern __shared__ __align__(16) int8_t xs[];   // [R][padded inner]
+  __shared__ T sh[2][W], sx[R];
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int k = (inner + 15) / 16 * 16;
+  {
+    const int r = w / PER, t = threadIdx.x - r * PER * 32;
+    const T* a = x + (int64_t)r * inner;
+    T top = T(0), odd = T(0);
+    if (r < rows) {
+#pragma unroll 4
+      for (int c = t; c < inner; c += PER * 32) {
+        const T v = fabs(a[c]);
+        top = fmax(top, v);
+        odd += v - v;
+      }
+    }
+    top = warp_max(top);
+    odd = warp_sum(odd);
+    if (lane == 0) {
+      sh[0][w] = top;
+      sh[1][w] = odd;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      top = fmax(top, sh[0][r * PER + i]);
+      odd += sh[1][r * PER + i];
+    }
+    const T scale = scale_of(top, odd);
+    const bool live = r < rows && scale > T(0);
+    const Reciprocal<T> by(scale);
+#pragma unroll 4
+    for (int c = t; c < k; c += PER * 32)
+      xs[r * k + c] = (int8_t)(live && c < inner ? by.of(a[c]) : 0);
+    if (t == 0) sx[r] = scale;
+    __syncthreads();
+  }
+  const int vecs = k / 16;
+  const int4* xv = reinterpret_cast<const int4*>(xs);
+  for (int64_t c0 = ((int64_t)blockIdx.x * W + w) * CH; c0 < outer;
+       c0 += (int64_t)gridDim.x * W * CH) {
+    int acc[CH][R] = {};
+#pragma unroll 2
+    for (int v = lane; v < vecs; v += 32) {
+      int4 wv[CH];
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        wv[c] = c0 + c < outer
+                    ? __ldg(reinterpret_cast<const int4*>(weight + (c0 + c) * ld) + v)
+                    : int4{};
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int4 a = xv[r * vecs + v];
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+          acc[c][r] = __dp4a(a.x, wv[c].x, __dp4a(a.y, wv[c].y, __dp4a(a.z, wv[c].z,
+                      __dp4a(a.w, wv[c].w, acc[c][r]))));
+      }
+    }
+    int mine = 0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int total = __reduce_add_sync(0xffffffffu, acc[c][r]);
+        if (lane == r * CH + c) mine = total;
+      }
+    const int r = lane / CH;
+    const int64_t c = c0 + lane % CH;
+    if (lane < R * CH && r < rows && c < outer) {
+      const T v = (T)mine * (sx[r] * scales[c]);
+      y[r * outer + c] = bias ? v + bias[c] : v;
+    }
   }
 }
 
@@ -93,6 +262,46 @@ int8_tile_kernel(const int8_t* __restrict__ a, const int8_t* __restrict__ b, int
   }
 }
 
+// Up to 8 rows whose integers fit 64 KB of shared memory take the one-launch kernel.
+bool takes_few(int64_t rows, int64_t inner) {
+  return rows <= 8 && (rows > 4 ? 8 : (rows > 2 ? 4 : rows)) * padded(inner) <= 65536;
+}
+
+template <typename T, int R, int CH>
+int launch_few_as(const T* x, int rows, int inner, const int8_t* weight, int64_t ld,
+                  const T* scales, const T* bias, T* y, int64_t outer, cudaStream_t s) {
+  auto kernel = few_rows_kernel<T, R, CH>;
+  TG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536));
+  const int64_t per = kThreads / 32 * CH;
+  const int64_t blocks = (outer + per - 1) / per;
+  const dim3 grid((unsigned)(blocks < 148 * 4 ? blocks : 148 * 4));
+  TG_CUDA_TRY(launch_pdl(kernel, grid, dim3(kThreads), (size_t)(R * padded(inner)), s, x, rows,
+                         inner, weight, ld, scales, bias, y, outer));
+  return check_launch("int8_linear(few rows)");
+}
+
+// Channels to a warp at a time: more of them keep more loads in flight, as long as every
+// multiprocessor still has two blocks.
+template <typename T, int R>
+int launch_few_rows(const T* x, int rows, int inner, const int8_t* weight, int64_t ld,
+                    const T* scales, const T* bias, T* y, int64_t outer, cudaStream_t s) {
+  const int64_t warps = 2 * 148 * (kThreads / 32);
+  if (outer >= 4 * warps)
+    return launch_few_as<T, R, 4>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
+  if (outer >= 2 * warps)
+    return launch_few_as<T, R, 2>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
+  return launch_few_as<T, R, 1>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
+}
+
+template <typename T>
+int launch_few(const T* x, int rows, int inner, const int8_t* weight, int64_t ld, const T* scales,
+               const T* bias, T* y, int64_t outer, cudaStream_t s) {
+  if (rows == 1) return launch_few_rows<T, 1>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
+  if (rows == 2) return launch_few_rows<T, 2>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
+  if (rows <= 4) return launch_few_rows<T, 4>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
+  return launch_few_rows<T, 8>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace
@@ -107,9 +316,24 @@ int tg_int8_quantize_rows(int dtype, const void* x, int64_t rows, int64_t inner,
   TG_CHECK_ARG(rows >= 0 && inner >= 0 && ld >= inner, "int8_quantize_rows: bad sizes");
   if (rows == 0) return TG_OK;
   cudaStream_t s = as_stream(stream);
+  const dim3 grid(grid_for(rows, 1));
+  if (dtype == TG_F32 && inner % 4 == 0 && ld % 4 == 0 && ld - inner < 16 && ld <= 8192 &&
+      aligned16(x) && (reinterpret_cast<uintptr_t>(q) & 3) == 0) {
+    const int groups = (int)(inner / 4);
+    const int64_t ld4 = ld / 4;
+    auto go = [&](auto kernel) {
+      launch_pdl(kernel, grid, dim3(kThreads), 0, s, (const float4*)x, rows, groups, (char4*)q,
+                 ld4, (float*)scales);
+      return check_launch("int8_quantize_rows");
+    };
+    if (ld4 <= kThreads) return go(quantize_rows_vec4_kernel<1>);
+    if (ld4 <= 2 * kThreads) return go(quantize_rows_vec4_kernel<2>);
+    if (ld4 <= 4 * kThreads) return go(quantize_rows_vec4_kernel<4>);
+    return go(quantize_rows_vec4_kernel<8>);
+  }
   return TG_DISPATCH_FLOAT(dtype, T, [&] {
-    quantize_rows_kernel<T><<<grid_for(rows, 1), kThreads, 0, s>>>((const T*)x, rows, inner, q,
-                                                                  ld, (T*)scales);
+    launch_pdl(quantize_rows_kernel<T>, grid, dim3(kThreads), 0, s, (const T*)x, rows, inner, q,
+               ld, (T*)scales);
     return check_launch("int8_quantize_rows");
   });
 }
@@ -117,7 +341,7 @@ int tg_int8_quantize_rows(int dtype, const void* x, int64_t rows, int64_t inner,
 size_t tg_int8_linear_scratch_bytes(int dtype, int64_t rows, int64_t inner, int64_t outer) {
   (void)outer;
   const size_t es = dtype == TG_F64 ? 8 : 4;
-  if (rows <= 0 || inner < 0) return 16;
+  if (rows <= 0 || inner <= 0 || takes_few(rows, inner)) return 16;
   return (size_t)(rows * padded(inner) + 255) / 256 * 256 + (size_t)rows * es + 256;
 }
 
@@ -131,14 +355,22 @@ int tg_int8_linear(int dtype, const void* x, int64_t rows, int64_t inner, const 
     return set_error(TG_ERR_UNSUPPORTED, "int8_linear: inner %lld (at most %lld, so that the "
                      "integer sums fit 32 bits)", (long long)inner, (long long)kMaxInner);
   if (rows == 0 || outer == 0) return TG_OK;
-  TG_CHECK_ARG(scratch && aligned16(scratch) && aligned16(weight),
-               "int8_linear: scratch and weight start on 16-byte boundaries");
+  TG_CHECK_ARG(weight && aligned16(weight), "int8_linear: the weight starts on a 16-byte boundary");
   cudaStream_t s = as_stream(stream);
+  if (takes_few(rows, inner))
+    return TG_DISPATCH_FLOAT(dtype, T, [&] {
+      return launch_few<T>((const T*)x, (int)rows, (int)inner, weight, ld, (const T*)scales,
+                           (const T*)bias, (T*)y, outer, s);
+    });
+  TG_CHECK_ARG(scratch && aligned16(scratch), "int8_linear: no scratch");
   const int64_t k = padded(inner);
   int8_t* q = reinterpret_cast<int8_t*>(scratch);
   uint8_t* after = reinterpret_cast<uint8_t*>(scratch) + (rows * k + 255) / 256 * 256;
   const int rc = tg_int8_quantize_rows(dtype, x, rows, inner, q, k, after, stream);
   if (rc) return rc;
+  if (dtype == TG_F32)
+    return int8_gemm_tc(q, weight, ld, (const float*)after, (const float*)scales,
+                        (const float*)bias, (float*)y, rows, inner, outer, s);
   return TG_DISPATCH_FLOAT(dtype, T, [&] {
     TG_CHECK_ARG((rows + 63) / 64 <= 65535, "int8_linear: too many rows");
     const dim3 grid((unsigned)((outer + 63) / 64), (unsigned)((rows + 63) / 64));

@@ -112,12 +112,13 @@ def synchronize() -> None:
 
 
 def _raise_kernel_timeouts() -> None:
-    """The tensor-core GEMM and the fused attention kernels give up a pipeline wait after a
+    """The tensor-core GEMMs and the fused attention kernels give up a pipeline wait after a
     cycle budget (about two seconds) instead of hanging; they then record TG_ERR_TIMEOUT in
-    a device status word, drain and return without finishing their outputs. Both words are
+    a device status word, drain and return without finishing their outputs. The words are
     read (and cleared) at every host synchronisation, so such a step raises here."""
     failed = [name for name, fn in (("tensor-core GEMM", lib.tg_gemm_tc_status),
-                                    ("fused attention", lib.tg_attention_tc_status))
+                                    ("fused attention", lib.tg_attention_tc_status),
+                                    ("8-bit integer linear", lib.tg_int8_tc_status))
               if fn(1) != 0]
     if failed:
         raise RuntimeError(f"{' and '.join(failed)}: a bounded device-side wait ran out "
