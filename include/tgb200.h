@@ -330,15 +330,13 @@ int tg_cross_entropy_backward(int dtype, const void* logits, const int64_t* targ
  *   top_log_probs[row][k], top_ids[row][k]: the top_k largest entries' log probabilities and
  *                    classes in descending order, equal entries by ascending class, NaN last.
  * Entries of -inf have probability 0 and add nothing. A row of -inf alone, or with a NaN or
- * +inf, gives NaN (its top_ids stay distinct classes). top_k <= tg_token_log_probs_max_top().
- * `scratch`: tg_token_log_probs_scratch_bytes(dtype, rows, classes, top_k). */
+ * +inf, gives NaN (its top_ids stay distinct classes). top_k <= tg_token_log_probs_max_top(),
+ * classes <= 2^30. */
 int tg_token_log_probs_max_top(void);
-size_t tg_token_log_probs_scratch_bytes(int dtype, int64_t rows, int64_t classes, int64_t top_k);
 int tg_token_log_probs_forward(int dtype, const void* logits, const int64_t* targets, void* stats,
                                void* log_probs, void* entropy, void* top_log_probs,
                                int64_t* top_ids, int64_t rows, int64_t classes, int64_t top_k,
-                               int64_t ignore_index, int* bad_target_dev, void* scratch,
-                               void* stream);
+                               int64_t ignore_index, int* bad_target_dev, void* stream);
 /* grad[row][j] = g_log[row] [j == t] + sum_k g_top[row][k] [j == top_ids[row][k]]
  *   - p_j (g_log[row] + sum_k g_top[row][k] + g_ent[row] (log p_j + entropy[row])). */
 int tg_token_log_probs_backward(int dtype, const void* logits, const int64_t* targets,

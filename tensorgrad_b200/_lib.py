@@ -145,8 +145,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tg_cross_entropy_backward": (c_int, [c_int, vp, vp, vp, vp, vp, vp, i64, i64, i64, c_int,
                                           vp]),
     "tg_token_log_probs_max_top": (c_int, []),
-    "tg_token_log_probs_scratch_bytes": (sz, [c_int, i64, i64, i64]),
-    "tg_token_log_probs_forward": (c_int, [c_int] + [vp] * 7 + [i64] * 4 + [vp] * 3),
+    "tg_token_log_probs_forward": (c_int, [c_int] + [vp] * 7 + [i64] * 4 + [vp] * 2),
     "tg_token_log_probs_backward": (c_int, [c_int] + [vp] * 9 + [i64] * 4 + [vp]),
     "tg_attention_forward_scratch_bytes": (sz, [c_int, POINTER(AttnShape)]),
     "tg_attention_forward": (c_int, [c_int, POINTER(AttnShape), vp, vp, vp, vp, vp, vp, vp]),

@@ -5,6 +5,8 @@
 //   (log p_i, i) of the k largest x_i, equal ones by ascending i
 // and their VJP. Row statistics m and s are kept apart for the VJP (p = e^(x - m) / s): folding
 // them into one log-sum-exp would round p to that sum's spacing.
+#include <cooperative_groups.h>
+
 #include <limits>
 
 #include "common.cuh"
@@ -14,6 +16,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTop = 128;
+constexpr int64_t kMaxClasses = 1 << 30;
 
 // ---------------------------------------------------------------- order of the alternatives
 // A value's place in the order as an unsigned key: larger value, larger key; both zeros alike;
@@ -53,38 +56,58 @@ __device__ __forceinline__ bool before(Alt<U> a, Alt<U> b) {
 }
 
 // ---------------------------------------------------------------- row statistics
-// Running maximum m, s = sum e^(x - m) and u = sum e^(x - m) (x - m).
+// Running maximum m (the type's lowest value before the first), s = sum e^(x - m) and
+// u = sum e^(x - m) (x - m).
 template <typename T>
 struct Stats {
   T m, s, u;
 };
 
-// The statistics of two sets of values as one. Shifting a maximum from m to m' >= m scales
-// every e^(x - m) by c = e^(m - m') and moves every x - m by m - m'.
+template <typename T>
+constexpr T kLowest = std::numeric_limits<T>::lowest();
+
+// e^x for x <= 0. The float form multiplies by log2 e in the argument: off by (4 + 2.4 |x|) half
+// steps, and a term of size |x| weighs e^x.
+__device__ __forceinline__ float exp_below(float x) { return __expf(x); }
+__device__ __forceinline__ double exp_below(double x) { return exp(x); }
+
+// The statistics of two sets of values as one. Shifting a maximum from m to m' >= m scales every
+// e^(x - m) by c = e^(m - m') and moves every x - m by m - m'.
 template <typename T>
 __device__ __forceinline__ Stats<T> join(Stats<T> a, Stats<T> b) {
-  const T m = fmax(a.m, b.m);
-  if (m == T(-INFINITY)) return {m, a.s + b.s, a.u + b.u};
-  Stats<T> r{m, T(0), T(0)};
-  const T da = a.m - m, db = b.m - m;
+  Stats<T> r{fmax(a.m, b.m), T(0), T(0)};
   if (a.s != T(0)) {
-    const T c = dev_exp<T>(da);
+    const T d = a.m - r.m, c = exp_below(d);
     r.s += a.s * c;
-    r.u += c * (a.u + (da == T(-INFINITY) ? T(0) : a.s * da));
+    r.u += c * (a.u + a.s * d);
   }
   if (b.s != T(0)) {
-    const T c = dev_exp<T>(db);
+    const T d = b.m - r.m, c = exp_below(d);
     r.s += b.s * c;
-    r.u += c * (b.u + (db == T(-INFINITY) ? T(0) : b.s * db));
+    r.u += c * (b.u + b.s * d);
   }
   return r;
 }
 
-// One more value. A value of -inf adds nothing; NaN and +inf make s and u NaN.
-template <typename T>
-__device__ __forceinline__ void push(Stats<T>& a, T x) {
-  if (x == T(-INFINITY)) return;
-  a = join(a, Stats<T>{x, x - x + T(1), x - x});
+// N more values at a time: the maximum moves at most once, each value costs one exponential. A
+// value of -inf adds nothing (0 times the lowest value); NaN and +inf make s NaN.
+template <int N, typename T>
+__device__ __forceinline__ void push(Stats<T>& a, const T (&x)[N]) {
+  T top = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) top = fmax(top, x[i]);
+  if (top > a.m) {
+    const T d = a.m - top, c = exp_below(d);
+    a.u = a.s != T(0) ? c * (a.u + a.s * d) : T(0);
+    a.s *= c;
+    a.m = top;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const T z = x[i] - a.m, e = exp_below(z);
+    a.s += e;
+    a.u += e * fmax(z, kLowest<T>);
+  }
 }
 
 template <typename T>
@@ -96,22 +119,42 @@ __device__ __forceinline__ Stats<T> block_join(Stats<T> a, Stats<T>* sh) {
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = a;
   __syncthreads();
   Stats<T> r = sh[0];
+#pragma unroll
   for (int i = 1; i < kThreads / 32; ++i) r = join(r, sh[i]);
-  __syncthreads();
   return r;
 }
 
-// The alternatives of a row one by one: each round takes the first one after the last found.
+template <typename T, int VE>
+struct alignas(sizeof(T) * VE) Vec {
+  T v[VE];
+};
+
+// ---------------------------------------------------------------- the alternatives
+constexpr int kList = 1024;  // entries that are ranked against each other
+
 template <typename T>
-__device__ void select_rounds(const T* __restrict__ x, int64_t classes, int top_k, T m, T ls,
-                              T* __restrict__ top, int64_t* __restrict__ ids) {
+struct Shared {
   using U = typename OrderKey<T>::U;
-  __shared__ Alt<U> best[kThreads / 32];
+  Stats<T> stats[kThreads / 32];
+  Stats<T> mine;            // the block's, for the cluster
+  Alt<U> list[kList];       // candidates
+  Alt<U> best[kMaxTop];     // the block's alternatives in order
+  U tops[kThreads];         // every lane's largest value
+  U bound;                  // no entry below it is an alternative
+  int count;
+};
+
+// The alternatives of values [0, n) one by one: each round takes the first one after the last
+// found. Always right and slow: for rows that have too many equal entries to list.
+template <typename T>
+__device__ void select_rounds(const T* __restrict__ x, int n, int first, int top_k,
+                              Shared<T>& sh) {
+  using U = typename OrderKey<T>::U;
   Alt<U> last{std::numeric_limits<U>::max(), -1};
   for (int k = 0; k < top_k; ++k) {
     Alt<U> mine{0, std::numeric_limits<int>::max()};
-    for (int64_t c = threadIdx.x; c < classes; c += kThreads) {
-      const Alt<U> a{OrderKey<T>::of(x[c]), (int)c};
+    for (int c = threadIdx.x; c < n; c += kThreads) {
+      const Alt<U> a{OrderKey<T>::of(x[c]), first + c};
       if (before(last, a) && before(a, mine)) mine = a;
     }
 #pragma unroll
@@ -120,81 +163,253 @@ __device__ void select_rounds(const T* __restrict__ x, int64_t classes, int top_
                          __shfl_xor_sync(0xffffffffu, mine.id, o)};
       if (before(other, mine)) mine = other;
     }
-    if ((threadIdx.x & 31) == 0) best[threadIdx.x >> 5] = mine;
     __syncthreads();
-    last = best[0];
+    if ((threadIdx.x & 31) == 0) sh.list[threadIdx.x >> 5] = mine;
+    __syncthreads();
+    last = sh.list[0];
     for (int i = 1; i < kThreads / 32; ++i)
-      if (before(best[i], last)) last = best[i];
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      top[k] = (x[last.id] - m) - ls;
-      ids[k] = last.id;
-    }
+      if (before(sh.list[i], last)) last = sh.list[i];
+    if (threadIdx.x == 0) sh.best[k] = last;
+  }
+  __syncthreads();
+}
+
+// The first top_k of n listed entries in order: an entry's place is how many come before it.
+template <typename T, typename F>
+__device__ __forceinline__ void rank_list(int n, int top_k, const Shared<T>& sh, F place) {
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const auto a = sh.list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += before(sh.list[j], a);
+    if (rank < top_k) place(rank, a);
   }
 }
 
+// The block's alternatives into sh.best, from every lane's largest value. The top_k-th largest of
+// those bounds the top_k-th largest value from below, and only lanes that reach it have entries
+// to look at again: about top_k of the row's kThreads-th parts are read twice.
+template <typename T, int VE>
+__device__ void select_top(const T* __restrict__ x, int n, int first, int top_k, T lane_top,
+                           Shared<T>& sh) {
+  using U = typename OrderKey<T>::U;
+  const U key = OrderKey<T>::of(lane_top), none = OrderKey<T>::of(kLowest<T>);
+  sh.tops[threadIdx.x] = key;
+  if (threadIdx.x == 0) sh.count = 0;
+  __syncthreads();
+  int rank = 0;
+#pragma unroll 8
+  for (int i = 0; i < kThreads; ++i) {
+    const U other = sh.tops[i];
+    rank += other > key || (other == key && i < (int)threadIdx.x);
+  }
+  if (rank == top_k - 1) sh.bound = key;
+  __syncthreads();
+  U bound = sh.bound;
+  if (bound <= none) {
+    // Fewer lanes than alternatives have a value: list everything, or go the slow way.
+    if (n > kList) {
+      select_rounds(x, n, first, top_k, sh);
+      return;
+    }
+    bound = 0;
+  }
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int units = n / VE;
+  for (int q = w; q < kThreads; q += kThreads / 32) {
+    if (bound != 0 && sh.tops[q] < bound) continue;
+    for (int i = q + lane * kThreads; i < units; i += 32 * kThreads) {
+      const Vec<T, VE> v = reinterpret_cast<const Vec<T, VE>*>(x)[i];
+#pragma unroll
+      for (int c = 0; c < VE; ++c) {
+        const U k = OrderKey<T>::of(v.v[c]);
+        if (k < bound) continue;
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kList) sh.list[at] = {k, first + i * VE + c};
+      }
+    }
+  }
+  __syncthreads();
+  const int found = sh.count;
+  if (found > kList) {
+    select_rounds(x, n, first, top_k, sh);
+    return;
+  }
+  rank_list(found, top_k, sh, [&](int rank, Alt<U> a) { sh.best[rank] = a; });
+  __syncthreads();
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-scores_fwd_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targets,
-                  T* __restrict__ stats, T* __restrict__ log_probs, T* __restrict__ entropy,
-                  T* __restrict__ top, int64_t* __restrict__ ids, int64_t rows, int64_t classes,
-                  int top_k, int64_t ignore_index, int* __restrict__ bad_target) {
-  __shared__ Stats<T> sh[kThreads / 32];
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const T* x = logits + r * classes;
-    Stats<T> a{T(-INFINITY), T(0), T(0)};
-    for (int64_t c = threadIdx.x; c < classes; c += kThreads) push(a, x[c]);
-    a = block_join(a, sh);
-    const T ls = dev_log<T>(a.s);
+struct ScoreArgs {
+  const T* logits;
+  const int64_t* targets;
+  T* stats;
+  T* log_probs;
+  T* entropy;
+  T* top;
+  int64_t* ids;
+  int64_t rows;
+  int classes, top_k, splits, part;  // part: classes of a split, a multiple of VE
+  int64_t ignore_index;
+  int* bad_target;
+};
+
+// One block a row, or a cluster of `splits` blocks with a part of its classes each. HBM-bound: one
+// read of the logits, VE of them to a load; 8 instructions and one exponential a value.
+template <typename T, int VE>
+__global__ void __launch_bounds__(kThreads, 4)
+scores_fwd_kernel(ScoreArgs<T> a) {
+  using U = typename OrderKey<T>::U;
+  constexpr int N = 2;  // loads in a step
+  __shared__ Shared<T> sh;
+  pdl_trigger();
+  pdl_wait();
+  const int split = blockIdx.x % a.splits;
+  for (int64_t r = blockIdx.x / a.splits; r < a.rows; r += gridDim.x / a.splits) {
+    const int first = split * a.part;
+    const int n = a.classes - first < a.part ? a.classes - first : a.part;
+    const T* row = a.logits + r * a.classes;
+    const T* x = row + first;
+    Stats<T> mine{kLowest<T>, T(0), T(0)};
+    const int units = n / VE;  // parts are multiples of VE
+    const Vec<T, VE>* xv = reinterpret_cast<const Vec<T, VE>*>(x);
+    int c = threadIdx.x;
+#pragma unroll 2
+    for (; c + (N - 1) * kThreads < units; c += N * kThreads) {
+      T v[N * VE];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const Vec<T, VE> y = xv[c + i * kThreads];
+#pragma unroll
+        for (int e = 0; e < VE; ++e) v[i * VE + e] = y.v[e];
+      }
+      push(mine, v);
+    }
+    for (; c < units; c += kThreads) {
+      const Vec<T, VE> y = xv[c];
+      push(mine, y.v);
+    }
+    const T lane_top = mine.m;
+    mine = block_join(mine, sh.stats);
+    if (a.top_k > 0) select_top<T, VE>(x, n, first, a.top_k, lane_top, sh);
+    if (a.splits > 1) {
+      const auto cluster = cooperative_groups::this_cluster();
+      if (threadIdx.x == 0) sh.mine = mine;
+      cluster.sync();
+      mine = *cluster.map_shared_rank(&sh.mine, 0);
+      for (int i = 1; i < a.splits; ++i) mine = join(mine, *cluster.map_shared_rank(&sh.mine, i));
+      if (split == 0) {
+        for (int i = threadIdx.x; i < a.splits * a.top_k; i += kThreads)
+          sh.list[i] = cluster.map_shared_rank(sh.best, i / a.top_k)[i % a.top_k];
+      }
+      cluster.sync();  // the others' results have been read
+    }
+    if (split != 0) continue;
+    const T ls = dev_log<T>(mine.s);
+    const T m = mine.s != T(0) ? mine.m : T(-INFINITY);  // a closed row has no log probabilities
+    auto place = [&](int rank, Alt<U> e) {
+      a.top[r * a.top_k + rank] = (row[e.id] - m) - ls;
+      a.ids[r * a.top_k + rank] = e.id;
+    };
+    if (a.splits > 1) {
+      rank_list(a.splits * a.top_k, a.top_k, sh, place);
+    } else {
+      for (int k = threadIdx.x; k < a.top_k; k += kThreads) place(k, sh.best[k]);
+    }
     if (threadIdx.x == 0) {
-      stats[2 * r] = a.m;
-      stats[2 * r + 1] = a.s;
-      entropy[r] = ls - a.u / a.s;
-      const int64_t t = targets[r];
+      a.stats[2 * r] = m;
+      a.stats[2 * r + 1] = mine.s;
+      a.entropy[r] = ls - mine.u / mine.s;
+      const int64_t t = a.targets[r];
       T lp = T(0);
-      if (t != ignore_index) {
-        if (t < 0 || t >= classes) {
-          if (bad_target) *bad_target = 1;
+      if (t != a.ignore_index) {
+        if (t < 0 || t >= a.classes) {
+          if (a.bad_target) *a.bad_target = 1;
         } else {
-          lp = (x[t] - a.m) - ls;
+          lp = (row[t] - m) - ls;
         }
       }
-      log_probs[r] = lp;
+      a.log_probs[r] = lp;
     }
-    if (top_k > 0)
-      select_rounds<T>(x, classes, top_k, a.m, ls, top + r * top_k, ids + r * top_k);
+    __syncthreads();
   }
 }
 
 // dx_j = -p_j (g_log + sum g_top + g_ent (log p_j + H)), then g_log at the target and g_top at
-// the alternatives.
-template <typename T>
+// the alternatives. Block (row, part of the classes); one read of the logits, one write.
+template <typename T, int VE>
 __global__ void __launch_bounds__(kThreads)
 scores_bwd_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targets,
                   const T* __restrict__ stats, const T* __restrict__ entropy,
                   const int64_t* __restrict__ ids, const T* __restrict__ g_log,
                   const T* __restrict__ g_ent, const T* __restrict__ g_top, T* __restrict__ grad,
-                  int64_t rows, int64_t classes, int top_k, int64_t ignore_index) {
+                  int64_t rows, int classes, int part, int top_k, int64_t ignore_index) {
+  pdl_trigger();
+  pdl_wait();
+  const int first = blockIdx.y * part;
+  const int n = classes - first < part ? classes - first : part;
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const T* x = logits + r * classes;
-    T* d = grad + r * classes;
+    const T* x = logits + r * classes + first;
+    T* d = grad + r * classes + first;
     const T m = stats[2 * r], s = stats[2 * r + 1];
     const T inv = T(1) / s, ls = dev_log<T>(s);
     const int64_t t = targets[r];
     const bool given = t != ignore_index && t >= 0 && t < classes;
-    const T gl = given ? g_log[r] : T(0), ge = g_ent[r], shift = entropy[r] - ls;
-    T push_all = gl;
-    for (int k = 0; k < top_k; ++k) push_all += g_top[r * top_k + k];
-    for (int64_t c = threadIdx.x; c < classes; c += kThreads) {
-      const T z = x[c] - m, p = dev_exp<T>(z) * inv;
-      // p = 0 leaves nothing, also where log p is -inf.
-      d[c] = p == T(0) ? T(0) : -p * (push_all + ge * (z + shift));
+    const T gl = given ? g_log[r] : T(0), ge = g_ent[r];
+    T tops = T(0);
+    for (int k = threadIdx.x & 31; k < top_k; k += 32) tops += g_top[r * top_k + k];
+    if (top_k > 0) tops = warp_sum(tops);
+    // -p (a + ge z) with z = x - m: log p + H = z + (H - log s).
+    const T a = gl + tops + ge * (entropy[r] - ls);
+    auto one = [&](T v) {
+      const T z = v - m, p = exp_below(z) * inv;
+      return p == T(0) ? T(0) : -p * (a + ge * z);  // nothing is left where log p may be -inf
+    };
+    const int units = n / VE;
+    const Vec<T, VE>* xv = reinterpret_cast<const Vec<T, VE>*>(x);
+    Vec<T, VE>* dv = reinterpret_cast<Vec<T, VE>*>(d);
+#pragma unroll 4
+    for (int c = threadIdx.x; c < units; c += kThreads) {
+      Vec<T, VE> v = xv[c];
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v.v[e] = one(v.v[e]);
+      dv[c] = v;
     }
+    // The single classes, by one lane each: the alternatives are distinct, the target may be
+    // one of them.
+    bool hit = false;
+    const int64_t at = t - first;
     __syncthreads();
-    if (threadIdx.x == 0 && given) d[t] += gl;
-    __syncthreads();
-    for (int k = threadIdx.x; k < top_k; k += kThreads) d[ids[r * top_k + k]] += g_top[r * top_k + k];
+    for (int k = threadIdx.x; k < top_k; k += kThreads) {
+      const int64_t i = ids[r * top_k + k] - first;
+      if (i < 0 || i >= n) continue;
+      const bool same = given && i == at;
+      hit |= same;
+      d[i] += g_top[r * top_k + k] + (same ? gl : T(0));
+    }
+    hit = __syncthreads_or(hit);
+    if (threadIdx.x == 0 && given && !hit && at >= 0 && at < n) d[at] += gl;
   }
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int sm_count() {
+  static int n = 0;
+  if (!n) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
+      n = 148;
+  }
+  return n;
+}
+
+// Parts of a row where the rows alone leave multiprocessors empty: up to 8 (a cluster), none
+// shorter than about 2048 classes, so that a part has more classes than alternatives are asked for.
+int row_splits(int64_t rows, int64_t classes) {
+  int s = 1;
+  while (s < 8 && rows * s < 2 * sm_count() && classes >= 2 * s * 2048) s *= 2;
+  return s;
 }
 
 }  // namespace
@@ -206,17 +421,11 @@ extern "C" {
 
 int tg_token_log_probs_max_top(void) { return kMaxTop; }
 
-size_t tg_token_log_probs_scratch_bytes(int dtype, int64_t rows, int64_t classes, int64_t top_k) {
-  return 16;
-}
-
 int tg_token_log_probs_forward(int dtype, const void* logits, const int64_t* targets, void* stats,
                                void* log_probs, void* entropy, void* top_log_probs,
                                int64_t* top_ids, int64_t rows, int64_t classes, int64_t top_k,
-                               int64_t ignore_index, int* bad_target_dev, void* scratch,
-                               void* stream) {
-  (void)scratch;
-  TG_CHECK_ARG(rows >= 0 && classes > 0 && classes <= INT32_MAX, "token_log_probs: bad shape");
+                               int64_t ignore_index, int* bad_target_dev, void* stream) {
+  TG_CHECK_ARG(rows >= 0 && classes > 0 && classes <= kMaxClasses, "token_log_probs: bad shape");
   TG_CHECK_ARG(top_k >= 0 && top_k <= kMaxTop && top_k <= classes,
                "token_log_probs: top_k %lld (at most %d and the %lld classes)", (long long)top_k,
                kMaxTop, (long long)classes);
@@ -224,10 +433,27 @@ int tg_token_log_probs_forward(int dtype, const void* logits, const int64_t* tar
   if (rows == 0) return TG_OK;
   cudaStream_t s = as_stream(stream);
   return TG_DISPATCH_FLOAT(dtype, T, [&] {
-    const unsigned grid = (unsigned)(rows < 148 * 16 ? rows : 148 * 16);
-    scores_fwd_kernel<T><<<grid, kThreads, 0, s>>>(
-        (const T*)logits, targets, (T*)stats, (T*)log_probs, (T*)entropy, (T*)top_log_probs,
-        top_ids, rows, classes, (int)top_k, ignore_index, bad_target_dev);
+    constexpr int VE = 16 / sizeof(T);
+    ScoreArgs<T> a{(const T*)logits, targets, (T*)stats, (T*)log_probs, (T*)entropy,
+                   (T*)top_log_probs, top_ids, rows, (int)classes, (int)top_k, 1, (int)classes,
+                   ignore_index, bad_target_dev};
+    a.splits = row_splits(rows, classes);
+    if (a.splits > 1) a.part = (int)((classes + a.splits * VE - 1) / (a.splits * VE) * VE);
+    const int64_t most = (int64_t)sm_count() * 8;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((rows < most ? rows : most) * a.splits));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim = {(unsigned)a.splits, 1, 1};
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    const bool vec = classes % VE == 0 && aligned16(logits);
+    TG_CUDA_TRY(vec ? cudaLaunchKernelEx(&cfg, scores_fwd_kernel<T, VE>, a)
+                    : cudaLaunchKernelEx(&cfg, scores_fwd_kernel<T, 1>, a));
     return check_launch("token_log_probs");
   });
 }
@@ -237,15 +463,22 @@ int tg_token_log_probs_backward(int dtype, const void* logits, const int64_t* ta
                                 const void* g_log, const void* g_ent, const void* g_top,
                                 void* grad, int64_t rows, int64_t classes, int64_t top_k,
                                 int64_t ignore_index, void* stream) {
-  TG_CHECK_ARG(rows >= 0 && classes > 0 && classes <= INT32_MAX && top_k >= 0 && top_k <= kMaxTop,
-               "token_log_probs backward: bad shape");
+  TG_CHECK_ARG(rows >= 0 && classes > 0 && classes <= kMaxClasses && top_k >= 0 &&
+                   top_k <= kMaxTop, "token_log_probs backward: bad shape");
   if (rows == 0) return TG_OK;
   cudaStream_t s = as_stream(stream);
   return TG_DISPATCH_FLOAT(dtype, T, [&] {
-    const unsigned grid = (unsigned)(rows < 148 * 16 ? rows : 148 * 16);
-    scores_bwd_kernel<T><<<grid, kThreads, 0, s>>>(
-        (const T*)logits, targets, (const T*)stats, (const T*)entropy, top_ids, (const T*)g_log,
-        (const T*)g_ent, (const T*)g_top, (T*)grad, rows, classes, (int)top_k, ignore_index);
+    constexpr int VE = 16 / sizeof(T);
+    const int parts = row_splits(rows, classes);
+    const int part = (int)((classes + parts * VE - 1) / (parts * VE) * VE);
+    const int64_t most = (int64_t)sm_count() * 8;
+    const dim3 grid((unsigned)(rows < most ? rows : most), (unsigned)parts);
+    const bool vec = classes % VE == 0 && aligned16(logits) && aligned16(grad);
+    TG_CUDA_TRY(launch_pdl(vec ? scores_bwd_kernel<T, VE> : scores_bwd_kernel<T, 1>, grid,
+                           dim3(kThreads), 0, s, (const T*)logits, targets, (const T*)stats,
+                           (const T*)entropy, top_ids, (const T*)g_log, (const T*)g_ent,
+                           (const T*)g_top, (T*)grad, rows, (int)classes, part, (int)top_k,
+                           ignore_index));
     return check_launch("token_log_probs backward");
   });
 }

@@ -9,6 +9,7 @@ import numpy as np
 
 from tensorgrad_b200 import device
 from tensorgrad_b200._lib import check, lib
+from tensorgrad_b200.autograd import is_grad_enabled
 from tensorgrad_b200.device import DeviceArray, dtype_code
 from tensorgrad_b200.ops import reduce
 from tensorgrad_b200.ops._util import (
@@ -264,23 +265,31 @@ def token_log_probs(logits: Any, targets: Any, *, top_k: int = 0,
     rows = math.prod(lead)
     code = dtype_code(x.dtype)
     es = x.itemsize
-    # One buffer: log probabilities, entropies, then (row, alternative) log probabilities.
-    packed = device.empty((rows * (2 + top_k),), x.dtype)
-    stats = device.empty((rows, 2), x.dtype)
+    # One buffer: log probabilities, entropies and (row, alternative) log probabilities, which
+    # are the result, then the rows' maxima and sums for the VJP.
+    size = rows * (2 + top_k)
+    whole = device.empty((size + 2 * rows,), x.dtype)
+    out, stats = whole.ptr, whole.ptr + size * es
     ids = device.empty((*lead, top_k), np.int64) if top_k else None
-    scratch = device.scratch(lib.tg_token_log_probs_scratch_bytes(code, rows, classes, top_k))
+    ids_ptr = ids.ptr if ids is not None else None
     check(lib.tg_token_log_probs_forward(
-        code, x.ptr, tgt.ptr, stats.ptr, packed.ptr, packed.ptr + rows * es,
-        packed.ptr + 2 * rows * es, ids.ptr if ids is not None else None, rows, classes, top_k,
-        ignore_index, bad, scratch.ptr, device.stream()), "token_log_probs")
+        code, x.ptr, tgt.ptr, stats, out, out + rows * es, out + 2 * rows * es, ids_ptr, rows,
+        classes, top_k, ignore_index, bad, device.stream()), "token_log_probs")
+    top_ids = Tensor._wrap(ids) if ids is not None else None
+    if not (tl.requires_grad and is_grad_enabled()):
+        return TokenLogProbs(
+            Tensor._wrap(whole.flat_view(0, rows, lead)),
+            Tensor._wrap(whole.flat_view(rows, rows, lead)),
+            None if ids is None else
+            Tensor._wrap(whole.flat_view(2 * rows, rows * top_k, ids.shape)), top_ids)
 
     def backward(g: DeviceArray, need: Need) -> tuple[DeviceArray]:
         if g.dtype != x.dtype:
             g = cast_array(g, x.dtype)
         grad = device.empty(tl.shape, x.dtype)
         check(lib.tg_token_log_probs_backward(
-            code, x.ptr, tgt.ptr, stats.ptr, packed.ptr + rows * es,
-            ids.ptr if ids is not None else None, g.ptr, g.ptr + rows * es, g.ptr + 2 * rows * es, grad.ptr, rows, classes, top_k,
+            code, x.ptr, tgt.ptr, whole.ptr + size * es, whole.ptr + rows * es, ids_ptr, g.ptr,
+            g.ptr + rows * es, g.ptr + 2 * rows * es, grad.ptr, rows, classes, top_k,
             ignore_index, device.stream()), "token_log_probs backward")
         return (grad if grad.dtype == tl.dtype else cast_array(grad, tl.dtype),)
 
@@ -289,11 +298,10 @@ def token_log_probs(logits: Any, targets: Any, *, top_k: int = 0,
                                                                      top_k, ignore_index),
                                   g, need)
 
-    whole = make_result(packed, (tl,), backward, "token_log_probs", graph)
+    packed = make_result(whole.flat_view(0, size), (tl,), backward, "token_log_probs", graph)
     return TokenLogProbs(
-        _part(whole, 0, lead), _part(whole, rows, lead),
-        _part(whole, 2 * rows, (*lead, top_k)) if ids is not None else None,
-        Tensor._wrap(ids) if ids is not None else None)
+        _part(packed, 0, lead), _part(packed, rows, lead),
+        None if ids is None else _part(packed, 2 * rows, ids.shape), top_ids)
 
 
 def _scores_composite(tl: Tensor, tgt: DeviceArray, ids: DeviceArray | None, rows: int,

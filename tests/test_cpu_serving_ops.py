@@ -49,7 +49,7 @@ def test_token_log_probs_entry_points_refuse_bad_sizes():
 
     def forward(rows, classes, top_k, dtype=0):
         return lib.tg_token_log_probs_forward(dtype, *[None] * 7, rows, classes, top_k, -100,
-                                              None, None, None)
+                                              None, None)
 
     assert forward(2, 0, 0) == 1
     assert forward(-1, 5, 0) == 1
