@@ -7,7 +7,6 @@
 //                    of ST stages, 128-byte swizzle.
 //   warp 1 (lane 0): MMA issuer (the pair's even CTA): four 32-byte steps a k-block into one of
 //                    two accumulators in tensor memory.
-//   warp 2 (lane 0): in a pair's odd CTA, tells the even one that a stage has landed here.
 //   warps 4..11    : epilogue, lane = row, two warps per lane quarter (one per half of the
 //                    columns): integers from tensor memory, scaled, through 32 x 32 boxes in
 //                    shared memory to TMA stores (rows of a multiple of 16 bytes) or plain ones.
@@ -15,6 +14,8 @@
 // 32768 products of a k column, a pair's 256 x 256 tile 256 bytes a CTA for the same.
 // Every wait is bounded; on expiry the kernel records TG_ERR_TIMEOUT in this unit's status word,
 // drains and frees its tensor memory.
+#include <initializer_list>
+
 #include "tc_ptx.cuh"
 
 namespace tg {
@@ -42,6 +43,7 @@ struct I8Layout {
 struct I8Args {
   int64_t rows, outer;
   int kblocks, tiles_m, tiles_n;
+  int a_rows;  // rows of A a copy brings: 128, or about the product's if it has fewer
   const float* row_scale;
   const float* scale;
   const float* bias;
@@ -80,6 +82,15 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y)
+      : "memory");
+}
+// The same, counted on a barrier of either CTA of the pair (its cluster address).
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar,
+                                                 int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
       : "memory");
 }
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x,
@@ -125,8 +136,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
-      // The producer's arrival and, in a pair's even CTA, the odd CTA's.
-      mbar_init(&full[s], PAIR && rank == 0 ? 2 : 1);
+      mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -161,9 +171,17 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           const int s = it % ST, round = it / ST;
           if (round > 0 && !wait_bar(&empty[s], (round - 1) & 1, abort_flag)) { stop = true; break; }
           uint8_t* st = smem + s * L::STAGE;
-          mbar_arrive_expect_tx(&full[s], L::STAGE);
-          tma_load_2d(st, &tmA, &full[s], j * kBK, m0);
-          tma_load_2d(st + L::A_BYTES, &tmB, &full[s], j * kBK, n0);
+          if constexpr (PAIR) {
+            // Both CTAs' copies count on the even CTA's barrier.
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * L::STAGE);
+            const uint32_t bar = map_to_rank(&full[s], 0);
+            tma_load_2d_pair(st, &tmA, bar, j * kBK, m0);
+            tma_load_2d_pair(st + L::A_BYTES, &tmB, bar, j * kBK, n0);
+          } else {
+            mbar_arrive_expect_tx(&full[s], (uint32_t)a.a_rows * kBK + L::B_BYTES);
+            tma_load_2d(st, &tmA, &full[s], j * kBK, m0);
+            tma_load_2d(st + L::A_BYTES, &tmB, &full[s], j * kBK, n0);
+          }
         }
       }
       // The copies in flight land, and the MMAs' last releases of the stages arrive, before the
@@ -171,19 +189,9 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       const bool aborted = *abort_flag != 0;
       for (int j = it - ST; j < it; ++j) {
         if (j < 0) continue;
-        if (aborted) wait_bar(&full[j % ST], (j / ST) & 1, abort_flag, false);
-        else wait_bar(&empty[j % ST], (j / ST) & 1, abort_flag);
+        if (aborted && rank == 0) wait_bar(&full[j % ST], (j / ST) & 1, abort_flag, false);
+        else if (!aborted) wait_bar(&empty[j % ST], (j / ST) & 1, abort_flag);
       }
-    }
-  } else if (PAIR && warp == 2) {
-    if (lane == 0 && rank == 1) {
-      int it = 0;
-      bool ok = true;
-      for (int t = unit; t < tiles && ok; t += units)
-        for (int j = 0; j < a.kblocks; ++j, ++it) {
-          if (!wait_bar(&full[it % ST], (it / ST) & 1, abort_flag)) { ok = false; break; }
-          mbar_arrive_cluster(map_to_rank(&full[it % ST], 0));
-        }
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
@@ -223,7 +231,8 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     const int quarter = warp & 3, half = (warp - kI8Epi0) >> 2;
     const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
     float4* box = reinterpret_cast<float4*>(staging + (warp - kI8Epi0) * kI8Box);
-    constexpr int CHUNKS = BN / 64;  // 32-column chunks of this warp's half
+    // 32-column chunks of this warp's half (a 32-wide tile is the first half's).
+    constexpr int CHUNKS = BN >= 64 ? BN / 64 : 1;
     int tc = 0;
     for (int t = unit; t < tiles; t += units, ++tc) {
       const int buf = tc & 1;
@@ -236,6 +245,10 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       tc_fence_after();
 #pragma unroll 1
       for (int c = 0; c < CHUNKS; ++c) {
+        if (BN < 64 && half == 1) {
+          if (lane == 0) mbar_arrive(&acc_empty[buf]);
+          break;
+        }
         const int col = (half * CHUNKS + c) * 32;
         const int64_t n0 = (int64_t)n * BN + col;
         uint32_t r[32];
@@ -323,7 +336,10 @@ int launch_i8(const int8_t* q, const int8_t* w, int64_t ld, I8Args a, int64_t k,
   using L = I8Layout<BN, PAIR>;
   CUtensorMap ma, mb, my;
   int rc;
-  if ((rc = i8_map(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, k, a.rows, k, kBK, 128))) return rc;
+  // A product of few rows leaves the rest of the tile's A rows as they are in shared memory: the
+  // accumulator rows that they make are never read.
+  a.a_rows = !PAIR && a.rows < 128 ? (int)((a.rows + 15) / 16 * 16) : 128;
+  if ((rc = i8_map(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, k, a.rows, k, kBK, a.a_rows))) return rc;
   if ((rc = i8_map(&mb, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, k, a.outer, ld, kBK, L::B_ROWS)))
     return rc;
   a.tma_y = a.outer % 4 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
@@ -367,7 +383,7 @@ int int8_gemm_tc(const int8_t* q, const int8_t* weight, int64_t ld, const float*
                  int64_t outer, cudaStream_t stream) {
   const int64_t k = (inner + 15) / 16 * 16;
   if (rows >= (int64_t)1 << 31 || outer >= (int64_t)1 << 31 ||
-      ((rows + 127) / 128) * ((outer + 63) / 64) >= (int64_t)1 << 30)
+      ((rows + 127) / 128) * ((outer + 31) / 32) >= (int64_t)1 << 30)
     return set_error(TG_ERR_UNSUPPORTED, "int8_linear: %lld x %lld outputs", (long long)rows,
                      (long long)outer);
   tc::I8Args a{};
@@ -378,12 +394,34 @@ int int8_gemm_tc(const int8_t* q, const int8_t* weight, int64_t ld, const float*
   a.scale = scales;
   a.bias = bias;
   a.y = y;
+  // What a multiprocessor is fed from the L2 a k-block decides (77 GB/s each, 11.4 TB/s together,
+  // measured alike for all widths): (A rows + BN) * 128 bytes a tile and k-block, times the rounds
+  // that the tiles take. Narrow tiles win where few would leave multiprocessors empty (512 x 768 x
+  // 2304: 64 wide 8.6 us, 128 wide 9.7, 256 wide 11.5), wide ones otherwise (4096 x 768 x 50304:
+  // 368, 268 and 255 us). A pair feeds 256 rows to a CTA for a 256-wide tile instead of 384, but
+  // costs a round more at its start and end: it wins on long reductions of several rounds (8192 x
+  // 4096 x 4096 130 against 142 us; 2048 x 768 x 2304 13.8 against 13.2).
   const int64_t tm = (rows + 127) / 128, sms = tc::sm_count();
-  if (tm * ((outer + 255) / 256) >= sms)
-    return tc::launch_i8<256, false>(q, weight, ld, a, k, stream);
-  if (tm * ((outer + 127) / 128) >= sms)
-    return tc::launch_i8<128, false>(q, weight, ld, a, k, stream);
-  return tc::launch_i8<64, false>(q, weight, ld, a, k, stream);
+  const int64_t pairs = (rows + 255) / 256 * ((outer + 255) / 256);
+  if (a.kblocks >= 16 && pairs > sms / 2)
+    return tc::launch_i8<256, true>(q, weight, ld, a, k, stream);
+  const int64_t a_rows = rows < 128 ? (rows + 15) / 16 * 16 : 128;
+  int best = 32;
+  int64_t least = INT64_MAX;
+  for (const int bn : {32, 64, 128, 256}) {
+    const int64_t rounds = (tm * ((outer + bn - 1) / bn) + sms - 1) / sms;
+    const int64_t cost = rounds * (a_rows + bn < 96 ? 96 : a_rows + bn);
+    if (cost < least) {
+      least = cost;
+      best = bn;
+    }
+  }
+  switch (best) {
+    case 32: return tc::launch_i8<32, false>(q, weight, ld, a, k, stream);
+    case 64: return tc::launch_i8<64, false>(q, weight, ld, a, k, stream);
+    case 128: return tc::launch_i8<128, false>(q, weight, ld, a, k, stream);
+  }
+  return tc::launch_i8<256, false>(q, weight, ld, a, k, stream);
 }
 
 }  // namespace tg

@@ -110,18 +110,23 @@ __device__ __forceinline__ void push(Stats<T>& a, const T (&x)[N]) {
   }
 }
 
-template <typename T>
-__device__ __forceinline__ Stats<T> block_join(Stats<T> a, Stats<T>* sh) {
+// Statistics over every group of LANES lanes.
+template <int LANES, typename T>
+__device__ __forceinline__ Stats<T> lanes_join(Stats<T> a) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
+  for (int o = LANES / 2; o > 0; o >>= 1)
     a = join(a, Stats<T>{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
                          __shfl_xor_sync(0xffffffffu, a.u, o)});
+  return a;
+}
+
+template <typename T>
+__device__ __forceinline__ Stats<T> block_join(Stats<T> a, Stats<T>* sh) {
+  static_assert(kThreads / 32 == 8, "one lane of a group of eight to a warp");
+  a = lanes_join<32>(a);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = a;
   __syncthreads();
-  Stats<T> r = sh[0];
-#pragma unroll
-  for (int i = 1; i < kThreads / 32; ++i) r = join(r, sh[i]);
-  return r;
+  return lanes_join<8>(sh[threadIdx.x & 7]);
 }
 
 template <typename T, int VE>
@@ -139,9 +144,10 @@ struct Shared {
   Stats<T> mine;            // the block's, for the cluster
   Alt<U> list[kList];       // candidates
   Alt<U> best[kMaxTop];     // the block's alternatives in order
-  U tops[kThreads];         // every lane's largest value
+  alignas(16) U tops[kThreads];  // every lane's largest value
+  int lanes[kThreads];      // those that reach the bound
   U bound;                  // no entry below it is an alternative
-  int count;
+  int count, lane_count;
 };
 
 // The alternatives of values [0, n) one by one: each round takes the first one after the last
@@ -180,6 +186,7 @@ __device__ __forceinline__ void rank_list(int n, int top_k, const Shared<T>& sh,
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const auto a = sh.list[i];
     int rank = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) rank += before(sh.list[j], a);
     if (rank < top_k) place(rank, a);
   }
@@ -192,17 +199,24 @@ template <typename T, int VE>
 __device__ void select_top(const T* __restrict__ x, int n, int first, int top_k, T lane_top,
                            Shared<T>& sh) {
   using U = typename OrderKey<T>::U;
+  constexpr U most = std::numeric_limits<U>::max();
   const U key = OrderKey<T>::of(lane_top), none = OrderKey<T>::of(kLowest<T>);
   sh.tops[threadIdx.x] = key;
-  if (threadIdx.x == 0) sh.count = 0;
-  __syncthreads();
-  int rank = 0;
-#pragma unroll 8
-  for (int i = 0; i < kThreads; ++i) {
-    const U other = sh.tops[i];
-    rank += other > key || (other == key && i < (int)threadIdx.x);
+  if (threadIdx.x == 0) {
+    sh.count = sh.lane_count = 0;
+    sh.bound = most;
   }
-  if (rank == top_k - 1) sh.bound = key;
+  __syncthreads();
+  // The top_k-th largest: the smallest that fewer than top_k others exceed.
+  int larger = 0;
+  const Vec<U, 16 / sizeof(U)>* tops = reinterpret_cast<const Vec<U, 16 / sizeof(U)>*>(sh.tops);
+#pragma unroll 8
+  for (int i = 0; i < kThreads * (int)sizeof(U) / 16; ++i) {
+    const auto others = tops[i];
+#pragma unroll
+    for (int e = 0; e < 16 / (int)sizeof(U); ++e) larger += others.v[e] > key;
+  }
+  if (larger < top_k) atomicMin(&sh.bound, key);
   __syncthreads();
   U bound = sh.bound;
   if (bound <= none) {
@@ -213,19 +227,19 @@ __device__ void select_top(const T* __restrict__ x, int n, int first, int top_k,
     }
     bound = 0;
   }
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int units = n / VE;
-  for (int q = w; q < kThreads; q += kThreads / 32) {
-    if (bound != 0 && sh.tops[q] < bound) continue;
-    for (int i = q + lane * kThreads; i < units; i += 32 * kThreads) {
-      const Vec<T, VE> v = reinterpret_cast<const Vec<T, VE>*>(x)[i];
+  if (key >= bound) sh.lanes[atomicAdd(&sh.lane_count, 1)] = threadIdx.x;
+  __syncthreads();
+  const int units = n / VE, each = (units + kThreads - 1) / kThreads, lanes = sh.lane_count;
+  for (int i = threadIdx.x; i < lanes * each; i += kThreads) {
+    const int c = sh.lanes[i / each] + i % each * kThreads;
+    if (c >= units) continue;
+    const Vec<T, VE> v = reinterpret_cast<const Vec<T, VE>*>(x)[c];
 #pragma unroll
-      for (int c = 0; c < VE; ++c) {
-        const U k = OrderKey<T>::of(v.v[c]);
-        if (k < bound) continue;
-        const int at = atomicAdd(&sh.count, 1);
-        if (at < kList) sh.list[at] = {k, first + i * VE + c};
-      }
+    for (int e = 0; e < VE; ++e) {
+      const U k = OrderKey<T>::of(v.v[e]);
+      if (k < bound) continue;
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kList) sh.list[at] = {k, first + c * VE + e};
     }
   }
   __syncthreads();
@@ -259,7 +273,7 @@ template <typename T, int VE>
 __global__ void __launch_bounds__(kThreads, 4)
 scores_fwd_kernel(ScoreArgs<T> a) {
   using U = typename OrderKey<T>::U;
-  constexpr int N = 2;  // loads in a step
+  constexpr int N = 4;  // loads in a step
   __shared__ Shared<T> sh;
   pdl_trigger();
   pdl_wait();
@@ -273,7 +287,7 @@ scores_fwd_kernel(ScoreArgs<T> a) {
     const int units = n / VE;  // parts are multiples of VE
     const Vec<T, VE>* xv = reinterpret_cast<const Vec<T, VE>*>(x);
     int c = threadIdx.x;
-#pragma unroll 2
+#pragma unroll 1
     for (; c + (N - 1) * kThreads < units; c += N * kThreads) {
       T v[N * VE];
 #pragma unroll
@@ -295,8 +309,9 @@ scores_fwd_kernel(ScoreArgs<T> a) {
       const auto cluster = cooperative_groups::this_cluster();
       if (threadIdx.x == 0) sh.mine = mine;
       cluster.sync();
-      mine = *cluster.map_shared_rank(&sh.mine, 0);
-      for (int i = 1; i < a.splits; ++i) mine = join(mine, *cluster.map_shared_rank(&sh.mine, i));
+      const int other = threadIdx.x & 7;
+      mine = lanes_join<8>(other < a.splits ? *cluster.map_shared_rank(&sh.mine, other)
+                                            : Stats<T>{kLowest<T>, T(0), T(0)});
       if (split == 0) {
         for (int i = threadIdx.x; i < a.splits * a.top_k; i += kThreads)
           sh.list[i] = cluster.map_shared_rank(sh.best, i / a.top_k)[i % a.top_k];

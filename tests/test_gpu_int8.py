@@ -29,7 +29,7 @@ def _quantized(x):
 
 def _check(y, x, q, scale, bias):
     a, s = _quantized(x)
-    total = a.astype(np.int64) @ q.astype(np.int64).T
+    total = a.astype(np.float64) @ q.astype(np.float64).T  # integers below 2^53: exact
     prod = total.astype(np.longdouble) * s[:, None].astype(np.longdouble) * scale.astype(np.longdouble)
     ref = prod if bias is None else prod + bias
     h = np.finfo(x.dtype).eps / 2
@@ -40,7 +40,8 @@ def _check(y, x, q, scale, bias):
 
 SHAPES = [(1, 1, 1), (1, 768, 2304), (7, 16, 1), (2, 17, 5), (8, 4096, 300), (9, 100, 70),
           (16, 768, 1000), (33, 1001, 77), (128, 64, 256), (129, 130, 65), (300, 4096, 513),
-          (1, 8192, 40), (2000, 256, 640), (1025, 48, 2052), (64, 2000, 129), (257, 1024, 4096)]
+          (1, 8192, 40), (2000, 256, 640), (1025, 48, 2052), (64, 2000, 129), (257, 1024, 4096),
+          (16, 4096, 4100), (2100, 130, 4500), (2049, 2100, 4100), (600, 3000, 8195)]
 
 
 @pytest.mark.parametrize("rows,inner,outer", SHAPES)
