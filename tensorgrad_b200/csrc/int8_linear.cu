@@ -136,25 +136,54 @@ quantize_rows_vec4_kernel(const float4* __restrict__ x, int groups,
 }
 
 // Up to R rows of input: every block quantises them into shared memory itself, then its warps
-// walk the output channels, CH at a time, 16 bytes of a weight row to a lane. One launch; what
-// bounds it is reading the weights once, and for small layers the launch.
-template <typename T, int R, int CH>
-__global__ void __launch_bounds__(kThreads)
+// walk the output channels, CH at a time, each lane with NV 16-byte groups of every one's weights
+// in flight and the next ones' behind them; the first are on their way before the input is
+// quantised. One launch. What bounds it is reading the weights once, and for small layers the
+// chain of launch, input, weights.
+template <typename T, int R, int CH, int NV, int FEW>
+__global__ void __launch_bounds__(FEW)
 few_rows_kernel(const T* __restrict__ x, int rows, int inner, const int8_t* __restrict__ weight,
                 int64_t ld, const T* __restrict__ scales, const T* __restrict__ bias,
                 T* __restrict__ y, int64_t outer) {
-  constexpr int W = kThreads / 32, PER = W / R;  // warps to a row
-  extern __shared__ __align__(16) int8_t xs[];   // [R][padded inner]
+  constexpr int W = FEW / 32, PER = W >= R ? W / R : 1;  // warps to a row
+  static_assert(W >= R, "a warp to a row");
+  extern __shared__ __align__(16) int8_t xs[];  // [R][padded inner]
   __shared__ T sh[2][W], sx[R];
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int k = (inner + 15) / 16 * 16;
+  const int k = (inner + 15) / 16 * 16, vecs = k / 16;
+  const int chunks = (vecs + 32 * NV - 1) / (32 * NV);
+  const int64_t stride = (int64_t)gridDim.x * W * CH;
+  int64_t c0 = ((int64_t)blockIdx.x * W + w) * CH;
+  auto load = [&](int4 (&to)[CH][NV], int64_t from, int chunk) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int v = (chunk * NV + i) * 32 + lane;
+        to[c][i] = v < vecs && from + c < outer
+                       ? __ldg(reinterpret_cast<const int4*>(weight + (from + c) * ld) + v)
+                       : int4{};
+      }
+  };
+  int4 wv[CH][NV];
+  load(wv, c0, 0);
   {
     const int r = w / PER, t = threadIdx.x - r * PER * 32;
     const T* a = x + (int64_t)r * inner;
     T top = T(0), odd = T(0);
-    if (r < rows) {
+    // Float rows of 16-byte groups go four values at a time.
+    const bool quads = sizeof(T) == 4 && inner % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+    if (r < rows && quads) {
+      const float4* a4 = reinterpret_cast<const float4*>(a);
+#pragma unroll 4
+      for (int c = t; c < inner / 4; c += PER * 32) {
+        const float4 v = a4[c];
+        top = fmax(top, (T)fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+        odd += (T)fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, v.w * 0.f)));
+      }
+    } else if (r < rows) {
 #pragma unroll 4
       for (int c = t; c < inner; c += PER * 32) {
         const T v = fabs(a[c]);
@@ -176,49 +205,65 @@ few_rows_kernel(const T* __restrict__ x, int rows, int inner, const int8_t* __re
     }
     const T scale = scale_of(top, odd);
     const bool live = r < rows && scale > T(0);
-    const Reciprocal<T> by(scale);
+    if (quads) {
+      const Reciprocal<float> by((float)scale);
+      const float4* a4 = reinterpret_cast<const float4*>(a);
 #pragma unroll 4
-    for (int c = t; c < k; c += PER * 32)
-      xs[r * k + c] = (int8_t)(live && c < inner ? by.of(a[c]) : 0);
+      for (int c = t; c < k / 4; c += PER * 32)
+        reinterpret_cast<char4*>(xs + r * k)[c] =
+            live && c < inner / 4 ? by.of4(a4[c]) : make_char4(0, 0, 0, 0);
+    } else {
+      const Reciprocal<T> by(scale);
+#pragma unroll 4
+      for (int c = t; c < k; c += PER * 32)
+        xs[r * k + c] = (int8_t)(live && c < inner ? by.of(a[c]) : 0);
+    }
     if (t == 0) sx[r] = scale;
     __syncthreads();
   }
-  const int vecs = k / 16;
   const int4* xv = reinterpret_cast<const int4*>(xs);
-  for (int64_t c0 = ((int64_t)blockIdx.x * W + w) * CH; c0 < outer;
-       c0 += (int64_t)gridDim.x * W * CH) {
-    int acc[CH][R] = {};
-#pragma unroll 2
-    for (int v = lane; v < vecs; v += 32) {
-      int4 wv[CH];
+  int acc[CH][R] = {};
+  for (int chunk = 0; c0 < outer;) {
+    int4 next[CH][NV];
+    const bool last = chunk + 1 == chunks;
+    load(next, last ? c0 + stride : c0, last ? 0 : chunk + 1);
 #pragma unroll
-      for (int c = 0; c < CH; ++c)
-        wv[c] = c0 + c < outer
-                    ? __ldg(reinterpret_cast<const int4*>(weight + (c0 + c) * ld) + v)
-                    : int4{};
+    for (int i = 0; i < NV; ++i) {
+      const int v = (chunk * NV + i) * 32 + lane;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const int4 a = xv[r * vecs + v];
+        const int4 a = v < vecs ? xv[r * vecs + v] : int4{};
 #pragma unroll
         for (int c = 0; c < CH; ++c)
-          acc[c][r] = __dp4a(a.x, wv[c].x, __dp4a(a.y, wv[c].y, __dp4a(a.z, wv[c].z,
-                      __dp4a(a.w, wv[c].w, acc[c][r]))));
+          acc[c][r] = __dp4a(a.x, wv[c][i].x, __dp4a(a.y, wv[c][i].y, __dp4a(a.z, wv[c][i].z,
+                      __dp4a(a.w, wv[c][i].w, acc[c][r]))));
       }
     }
-    int mine = 0;
+    if (last) {
+      int mine = 0;
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int total = __reduce_add_sync(0xffffffffu, acc[c][r]);
+          if (lane == r * CH + c) mine = total;
+          acc[c][r] = 0;
+        }
+      const int r = lane / CH;
+      const int64_t c = c0 + lane % CH;
+      if (lane < R * CH && r < rows && c < outer) {
+        const T v = (T)mine * (sx[r] * scales[c]);
+        y[r * outer + c] = bias ? v + bias[c] : v;
+      }
+      c0 += stride;
+      chunk = 0;
+    } else {
+      ++chunk;
+    }
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int total = __reduce_add_sync(0xffffffffu, acc[c][r]);
-        if (lane == r * CH + c) mine = total;
-      }
-    const int r = lane / CH;
-    const int64_t c = c0 + lane % CH;
-    if (lane < R * CH && r < rows && c < outer) {
-      const T v = (T)mine * (sx[r] * scales[c]);
-      y[r * outer + c] = bias ? v + bias[c] : v;
-    }
+      for (int i = 0; i < NV; ++i) wv[c][i] = next[c][i];
   }
 }
 
@@ -268,44 +313,60 @@ int8_tile_kernel(const int8_t* __restrict__ a, const int8_t* __restrict__ b, int
   }
 }
 
-// Up to 8 rows whose integers fit 64 KB of shared memory take the one-launch kernel.
-bool takes_few(int64_t rows, int64_t inner) {
-  return rows <= 8 && (rows > 4 ? 8 : (rows > 2 ? 4 : rows)) * padded(inner) <= 65536;
+// Up to 8 rows take the one-launch kernel, more than 2 of them only below 16384 channels: there its
+// multiplications cost more than the tensor cores' second launch (8 rows of 4096 through 4096
+// channels 12.2 us against 15.5, 6 of 2048 through 8192 8.2 against 10.5, 8 of 768 through 50304
+// 23.2 against 16.9; 2 rows 11.4 against 16.4).
+bool takes_few(int64_t rows, int64_t inner, int64_t outer) {
+  return rows <= 8 && (rows <= 2 || outer < 16384) &&
+         (rows > 4 ? 8 : (rows > 2 ? 4 : rows)) * padded(inner) <= 49152;
 }
 
-template <typename T, int R, int CH>
+template <typename T, int R, int CH, int NV>
 int launch_few_as(const T* x, int rows, int inner, const int8_t* weight, int64_t ld,
                   const T* scales, const T* bias, T* y, int64_t outer, cudaStream_t s) {
-  auto kernel = few_rows_kernel<T, R, CH>;
-  TG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536));
-  const int64_t per = kThreads / 32 * CH;
-  const int64_t blocks = (outer + per - 1) / per;
-  const dim3 grid((unsigned)(blocks < 148 * 4 ? blocks : 148 * 4));
-  TG_CUDA_TRY(launch_pdl(kernel, grid, dim3(kThreads), (size_t)(R * padded(inner)), s, x, rows,
-                         inner, weight, ld, scales, bias, y, outer));
+  // Every block quantises the input: short rows in many small blocks, long ones in few large.
+  constexpr int FEW = NV > 2 ? 512 : (R <= 4 ? 128 : 256), W = FEW / 32;
+  constexpr int64_t MOST = 148 * (NV <= 2 ? 6 : 1);
+  const int64_t blocks = (outer + W * CH - 1) / (W * CH);
+  const dim3 grid((unsigned)(blocks < MOST ? blocks : MOST));
+  TG_CUDA_TRY(launch_pdl(few_rows_kernel<T, R, CH, NV, FEW>, grid, dim3(FEW),
+                         (size_t)(R * padded(inner)), s, x, rows, inner, weight, ld, scales, bias,
+                         y, outer));
   return check_launch("int8_linear(few rows)");
 }
 
-// Channels to a warp at a time: more of them keep more loads in flight, as long as every
-// multiprocessor still has two blocks.
-template <typename T, int R>
+// Channels to a warp at a time: 8 loads in flight if the channels are many enough to give every
+// multiprocessor 8 warps all the same.
+template <typename T, int R, int NV>
 int launch_few_rows(const T* x, int rows, int inner, const int8_t* weight, int64_t ld,
                     const T* scales, const T* bias, T* y, int64_t outer, cudaStream_t s) {
-  const int64_t warps = 2 * 148 * (kThreads / 32);
-  if (outer >= 4 * warps)
-    return launch_few_as<T, R, 4>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
-  if (outer >= 2 * warps)
-    return launch_few_as<T, R, 2>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
-  return launch_few_as<T, R, 1>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
+  if constexpr (NV <= 2)
+    if (outer >= 4 * 148 * 8)
+      return launch_few_as<T, R, 4, NV>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
+  if constexpr (NV <= 4)
+    if (outer >= 2 * 148 * 8)
+      return launch_few_as<T, R, 2, NV>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
+  return launch_few_as<T, R, 1, NV>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
+}
+
+template <typename T, int R>
+int launch_few_inner(const T* x, int rows, int inner, const int8_t* weight, int64_t ld,
+                     const T* scales, const T* bias, T* y, int64_t outer, cudaStream_t s) {
+  if (inner <= 1024)
+    return launch_few_rows<T, R, 2>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
+  if (inner <= 2048)
+    return launch_few_rows<T, R, 4>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
+  return launch_few_rows<T, R, 8>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
 }
 
 template <typename T>
 int launch_few(const T* x, int rows, int inner, const int8_t* weight, int64_t ld, const T* scales,
                const T* bias, T* y, int64_t outer, cudaStream_t s) {
-  if (rows == 1) return launch_few_rows<T, 1>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
-  if (rows == 2) return launch_few_rows<T, 2>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
-  if (rows <= 4) return launch_few_rows<T, 4>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
-  return launch_few_rows<T, 8>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
+  if (rows == 1) return launch_few_inner<T, 1>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
+  if (rows == 2) return launch_few_inner<T, 2>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
+  if (rows <= 4) return launch_few_inner<T, 4>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
+  return launch_few_inner<T, 8>(x, rows, inner, weight, ld, scales, bias, y, outer, s);
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -346,9 +407,8 @@ int tg_int8_quantize_rows(int dtype, const void* x, int64_t rows, int64_t inner,
 }
 
 size_t tg_int8_linear_scratch_bytes(int dtype, int64_t rows, int64_t inner, int64_t outer) {
-  (void)outer;
   const size_t es = dtype == TG_F64 ? 8 : 4;
-  if (rows <= 0 || inner <= 0 || takes_few(rows, inner)) return 16;
+  if (rows <= 0 || inner <= 0 || takes_few(rows, inner, outer)) return 16;
   return (size_t)(rows * padded(inner) + 255) / 256 * 256 + (size_t)rows * es + 256;
 }
 
@@ -364,7 +424,7 @@ int tg_int8_linear(int dtype, const void* x, int64_t rows, int64_t inner, const 
   if (rows == 0 || outer == 0) return TG_OK;
   TG_CHECK_ARG(weight && aligned16(weight), "int8_linear: the weight starts on a 16-byte boundary");
   cudaStream_t s = as_stream(stream);
-  if (takes_few(rows, inner))
+  if (takes_few(rows, inner, outer))
     return TG_DISPATCH_FLOAT(dtype, T, [&] {
       return launch_few<T>((const T*)x, (int)rows, (int)inner, weight, ld, (const T*)scales,
                            (const T*)bias, (T*)y, outer, s);
