@@ -10,6 +10,7 @@
 #include <cooperative_groups.h>
 
 #include <limits>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -17,107 +18,6 @@ namespace tg {
 namespace {
 
 constexpr int kThreads = 256;
-
-struct Pool {
-  int64_t num_pages, kv_heads, page_size, head_dim;  // head_dim in units of the element moved
-  const int64_t* table;                              // (batch, max_pages)
-  int64_t max_pages;
-  int* bad;
-};
-
-// The position's row of one head in a pool, or -1 behind a bad id or off the table.
-__device__ __forceinline__ int64_t row_of(const Pool& p, int64_t b, int64_t h, int64_t at) {
-  const int64_t slot = at / p.page_size;
-  if (at < 0 || slot >= p.max_pages) {
-    if (p.bad) *p.bad = 1;
-    return -1;
-  }
-  const int64_t page = p.table[b * p.max_pages + slot];
-  if (page < 0 || page >= p.num_pages) {
-    if (p.bad) *p.bad = 1;
-    return -1;
-  }
-  return ((page * p.kv_heads + h) * p.page_size + at % p.page_size) * p.head_dim;
-}
-
-__device__ __forceinline__ int64_t length_of(const Pool& p, const int64_t* lengths, int64_t b) {
-  const int64_t n = lengths[b], most = p.max_pages * p.page_size;
-  if (n < 0 || n > most) {
-    if (p.bad) *p.bad = 1;
-    return n < 0 ? 0 : most;
-  }
-  return n;
-}
-
-// ---------------------------------------------------------------- append, gather, copy
-// V: the unit moved (an element, or 16 bytes where widths, strides and addresses allow).
-struct Rows {
-  int64_t sb, sh, st;  // strides of (batch, head, position) in units
-};
-
-template <typename V>
-__global__ void __launch_bounds__(kThreads)
-append_kernel(Pool p, int64_t batch, int64_t tokens, const V* __restrict__ k, Rows ks,
-              const V* __restrict__ v, Rows vs, const int64_t* __restrict__ start,
-              V* __restrict__ keys, V* __restrict__ values) {
-  const int64_t total = batch * tokens * p.kv_heads * p.head_dim;
-  for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < total;
-       e += (int64_t)gridDim.x * kThreads) {
-    const int64_t c = e % p.head_dim, r = e / p.head_dim;
-    const int64_t t = r % tokens, bh = r / tokens, h = bh % p.kv_heads, b = bh / p.kv_heads;
-    const int64_t to = start[b] < 0 ? row_of(p, b, h, -1) : row_of(p, b, h, start[b] + t);
-    if (to < 0) continue;
-    keys[to + c] = k[b * ks.sb + h * ks.sh + t * ks.st + c];
-    values[to + c] = v[b * vs.sb + h * vs.sh + t * vs.st + c];
-  }
-}
-
-template <typename V>
-__global__ void __launch_bounds__(kThreads)
-gather_kernel(Pool p, int64_t batch, int64_t longest, const V* __restrict__ keys,
-              const V* __restrict__ values, const int64_t* __restrict__ lengths,
-              V* __restrict__ k, V* __restrict__ v) {
-  const int64_t total = batch * p.kv_heads * longest * p.head_dim;
-  for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < total;
-       e += (int64_t)gridDim.x * kThreads) {
-    const int64_t c = e % p.head_dim, r = e / p.head_dim;
-    const int64_t t = r % longest, bh = r / longest, h = bh % p.kv_heads, b = bh / p.kv_heads;
-    const int64_t from = t < length_of(p, lengths, b) ? row_of(p, b, h, t) : -1;
-    k[e] = from < 0 ? V{} : keys[from + c];
-    v[e] = from < 0 ? V{} : values[from + c];
-  }
-}
-
-// Pages src[i] to dst[i] in every layer of both pools; `units` of V to a page.
-template <typename V>
-__global__ void __launch_bounds__(kThreads)
-page_copy_kernel(V* keys, V* values, int64_t layers, int64_t num_pages, int64_t units,
-                 const int64_t* __restrict__ src, const int64_t* __restrict__ dst, int64_t pairs,
-                 int* __restrict__ bad) {
-  const int64_t total = 2 * layers * pairs;
-  for (int64_t e = blockIdx.x; e < total; e += gridDim.x) {
-    const int64_t i = e % pairs, l = e / pairs;
-    const int64_t from = src[i], to = dst[i];
-    if (from < 0 || from >= num_pages || to < 0 || to >= num_pages) {
-      if (bad && threadIdx.x == 0) *bad = 1;
-      continue;
-    }
-    V* pool = (l < layers ? keys : values) + (l % layers) * num_pages * units;
-    const V* a = pool + from * units;
-    V* b = pool + to * units;
-    for (int64_t c = threadIdx.x; c < units; c += kThreads) b[c] = a[c];
-  }
-}
-
-// ---------------------------------------------------------------- attention of one token
-constexpr int kMaxHead = 256;
-constexpr int kAttend = 128;        // threads of an attention block
-constexpr int kWarps = kAttend / 32;
-constexpr int kLaneDims = 8;        // features of a position that one lane holds
-constexpr int kTable = 512;        // pages named in shared memory at a time
-constexpr int kMinSplit = 128;      // positions that a block has at least, if there are as many
-constexpr int kMaxSplits = 512;
-constexpr int kMaxCluster = 8;      // splits that join through their cluster's shared memory
 
 // n / d for 0 <= n < 2^31 by a multiplication (d fixed for a launch; Granlund and Montgomery,
 // "Division by invariant integers using multiplication", 1994).
@@ -132,6 +32,165 @@ FastDiv make_div(int64_t d) {
 __device__ __forceinline__ int div_by(int n, FastDiv f) {
   return (int)((__umulhi((uint32_t)n, f.mul) + (uint32_t)n) >> f.shift);
 }
+
+struct Pool {
+  int64_t num_pages, kv_heads, page_size, head_dim;  // head_dim in units of what is moved
+  const int64_t* table;                              // (batch, max_pages)
+  int64_t max_pages;
+  int* bad;
+};
+
+// The position's row of one head in a pool, or -1 behind a bad id or off the table.
+__device__ __forceinline__ int64_t row_of(const Pool& p, FastDiv size, int64_t b, int h,
+                                          int64_t at) {
+  if (at < 0 || at >= p.max_pages * p.page_size) {
+    if (p.bad) *p.bad = 1;
+    return -1;
+  }
+  const int slot = div_by((int)at, size);
+  const int64_t page = p.table[b * p.max_pages + slot];
+  if (page < 0 || page >= p.num_pages) {
+    if (p.bad) *p.bad = 1;
+    return -1;
+  }
+  return ((page * p.kv_heads + h) * p.page_size + ((int)at - slot * (int)size.d)) * p.head_dim;
+}
+
+__device__ __forceinline__ int64_t length_of(const Pool& p, const int64_t* lengths, int64_t b) {
+  const int64_t n = lengths[b], most = p.max_pages * p.page_size;
+  if (n < 0 || n > most) {
+    if (p.bad) *p.bad = 1;
+    return n < 0 ? 0 : most;
+  }
+  return n;
+}
+
+// ---------------------------------------------------------------- append, gather, copy
+// V: the unit moved (an element, or 16 bytes where widths, strides and addresses allow). LPR lanes
+// share a (sequence, head, position) row, its place is worked out once. HBM-bound: 16 x 12 heads
+// of 64 over 1024 positions appended at 5.3 TB/s, one sequence of 65536 gathered at 5.7.
+struct Rows {
+  int64_t sb, sh, st;  // strides of (batch, head, position) in units
+};
+
+struct Moves {
+  Pool pool;
+  int rows;                       // batch * heads * positions
+  FastDiv heads, positions, size;
+  const int64_t* lengths;
+};
+
+template <int LPR, typename F>
+__device__ __forceinline__ void each_row(const Moves& m, F body) {
+  const int lane = threadIdx.x % LPR;
+  const int step = (int)gridDim.x * (kThreads / LPR);
+  for (int r = blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR; r < m.rows; r += step) {
+    const int bh = div_by(r, m.positions), t = r - bh * (int)m.positions.d;
+    const int b = div_by(bh, m.heads), h = bh - b * (int)m.heads.d;
+    body(b, h, t, lane);
+  }
+}
+
+template <typename V, int LPR>
+__global__ void __launch_bounds__(kThreads)
+append_kernel(Moves m, const V* __restrict__ k, Rows ks, const V* __restrict__ v, Rows vs,
+              V* __restrict__ keys, V* __restrict__ values) {
+  each_row<LPR>(m, [&](int b, int h, int t, int lane) {
+    const int64_t start = m.lengths[b];
+    const int64_t to = row_of(m.pool, m.size, b, h, start < 0 ? -1 : start + t);
+    if (to < 0) return;
+    const V* a = k + b * ks.sb + h * ks.sh + t * ks.st;
+    const V* c = v + b * vs.sb + h * vs.sh + t * vs.st;
+    for (int i = lane; i < (int)m.pool.head_dim; i += LPR) {
+      keys[to + i] = a[i];
+      values[to + i] = c[i];
+    }
+  });
+}
+
+template <typename V, int LPR>
+__global__ void __launch_bounds__(kThreads)
+gather_kernel(Moves m, const V* __restrict__ keys, const V* __restrict__ values,
+              V* __restrict__ k, V* __restrict__ v) {
+  const int d = (int)m.pool.head_dim;
+  each_row<LPR>(m, [&](int b, int h, int t, int lane) {
+    const int64_t from =
+        t < length_of(m.pool, m.lengths, b) ? row_of(m.pool, m.size, b, h, t) : -1;
+    const int64_t to = (((int64_t)b * m.heads.d + h) * m.positions.d + t) * d;
+    for (int i = lane; i < d; i += LPR) {
+      k[to + i] = from < 0 ? V{} : keys[from + i];
+      v[to + i] = from < 0 ? V{} : values[from + i];
+    }
+  });
+}
+
+// Pages src[i] to dst[i] in every layer of both pools; `units` of V to a page. Pages of 256 units
+// and more take a block or several (1024 pages of 48 KB in 12 layers: 6.1 TB/s), shorter ones share
+// one.
+template <typename V>
+struct Copies {
+  V* keys;
+  V* values;
+  int64_t layers, num_pages, units;
+  const int64_t* src;
+  const int64_t* dst;
+  int64_t pairs;
+  int* bad;
+};
+
+// Where copy e of 2 layers pairs reads and writes; false behind a bad id.
+template <typename V>
+__device__ __forceinline__ bool place_of(const Copies<V>& c, int64_t l, int64_t i, const V*& from,
+                                         V*& to) {
+  const int64_t a = c.src[i], b = c.dst[i];
+  if (a < 0 || a >= c.num_pages || b < 0 || b >= c.num_pages) {
+    if (c.bad) *c.bad = 1;
+    return false;
+  }
+  V* pool = l < c.layers ? c.keys + l * c.num_pages * c.units
+                         : c.values + (l - c.layers) * c.num_pages * c.units;
+  from = pool + a * c.units;
+  to = pool + b * c.units;
+  return true;
+}
+
+template <typename V>
+__global__ void __launch_bounds__(kThreads)
+page_copy_kernel(Copies<V> c, int parts, int64_t part) {
+  const int64_t total = 2 * c.layers * c.pairs * parts;
+  for (int64_t e = blockIdx.x; e < total; e += gridDim.x) {
+    const int64_t p = e / parts, first = e % parts * part;
+    const int64_t end = first + part < c.units ? first + part : c.units;
+    const V* from;
+    V* to;
+    if (!place_of(c, p / c.pairs, p % c.pairs, from, to)) continue;
+#pragma unroll 4
+    for (int64_t i = first + threadIdx.x; i < end; i += kThreads) to[i] = from[i];
+  }
+}
+
+template <typename V>
+__global__ void __launch_bounds__(kThreads)
+page_copy_short_kernel(Copies<V> c, int total, FastDiv units, FastDiv pairs) {
+  for (int e = blockIdx.x * kThreads + threadIdx.x; e < total; e += (int)gridDim.x * kThreads) {
+    const int p = div_by(e, units), l = div_by(p, pairs);
+    const V* from;
+    V* to;
+    if (!place_of(c, l, p - l * (int)pairs.d, from, to)) continue;
+    const int i = e - p * (int)units.d;
+    to[i] = from[i];
+  }
+}
+
+// ---------------------------------------------------------------- attention of one token
+constexpr int kMaxHead = 256;
+constexpr int kAttend = 128;        // threads of an attention block
+constexpr int kWarps = kAttend / 32;
+constexpr int kLaneDims = 8;        // features of a position that one lane holds
+constexpr int kTable = 512;        // pages named in shared memory at a time
+constexpr int kMinSplit = 128;      // positions that a block has at least, if there are as many
+constexpr int kMaxSplits = 512;
+constexpr int kMaxCluster = 8;      // splits that join through their cluster's shared memory
 
 // e^x on scores that carry the factor `unit`: float scores are in base 2 (one instruction less
 // per weight), double ones in base e.
@@ -653,7 +712,71 @@ int check_pool(const char* what, int64_t num_pages, int64_t kv_heads, int64_t pa
                "%s: pool of %lld pages of (%lld heads, %lld positions, %lld features), table of "
                "%lld", what, (long long)num_pages, (long long)kv_heads, (long long)page_size,
                (long long)head_dim, (long long)max_pages);
+  TG_CHECK_ARG(num_pages <= INT32_MAX && kv_heads <= INT32_MAX && head_dim <= INT32_MAX &&
+                   max_pages <= (INT32_MAX - (1 << 16)) / page_size,
+               "%s: positions up to 2^31 (table of %lld pages of %lld)", what,
+               (long long)max_pages, (long long)page_size);
   return TG_OK;
+}
+
+// The rows of (batch, heads, positions), and how many blocks of LPR lanes a row they make.
+int make_moves(const char* what, const Pool& pool, int64_t batch, int64_t positions,
+               const int64_t* lengths, Moves& m) {
+  TG_CHECK_ARG(batch <= INT32_MAX / pool.kv_heads / positions, "%s: %lld x %lld x %lld rows", what,
+               (long long)batch, (long long)pool.kv_heads, (long long)positions);
+  m.pool = pool;
+  m.rows = (int)(batch * pool.kv_heads * positions);
+  m.heads = make_div(pool.kv_heads);
+  m.positions = make_div(positions);
+  m.size = make_div(pool.page_size);
+  m.lengths = lengths;
+  return TG_OK;
+}
+
+// Calls f with the lanes to a row of `units`: a power of two up to a warp.
+template <typename F>
+int with_lanes(int64_t units, F f) {
+  if (units <= 4) return f(std::integral_constant<int, 4>{});
+  if (units <= 8) return f(std::integral_constant<int, 8>{});
+  if (units <= 16) return f(std::integral_constant<int, 16>{});
+  return f(std::integral_constant<int, 32>{});
+}
+
+template <typename V>
+int launch_append(const Moves& m, const V* k, Rows ks, const V* v, Rows vs, V* keys, V* values,
+                  cudaStream_t s) {
+  return with_lanes(m.pool.head_dim, [&](auto lanes) {
+    constexpr int LPR = decltype(lanes)::value;
+    append_kernel<V, LPR><<<grid_for((int64_t)m.rows * LPR, kThreads), kThreads, 0, s>>>(
+        m, k, ks, v, vs, keys, values);
+    return check_launch("paged_append");
+  });
+}
+
+template <typename V>
+int launch_gather(const Moves& m, const V* keys, const V* values, V* k, V* v, cudaStream_t s) {
+  return with_lanes(m.pool.head_dim, [&](auto lanes) {
+    constexpr int LPR = decltype(lanes)::value;
+    gather_kernel<V, LPR><<<grid_for((int64_t)m.rows * LPR, kThreads), kThreads, 0, s>>>(
+        m, keys, values, k, v);
+    return check_launch("paged_gather");
+  });
+}
+
+template <typename V>
+int launch_copies(const Copies<V>& c, cudaStream_t s) {
+  const int64_t pages = 2 * c.layers * c.pairs;
+  if (c.units < kThreads && pages * c.units <= INT32_MAX / 2)
+    page_copy_short_kernel<V><<<grid_for(pages * c.units, kThreads), kThreads, 0, s>>>(
+        c, (int)(pages * c.units), make_div(c.units), make_div(c.pairs));
+  else {
+    // Few pages are cut into parts of at least 4 units a lane.
+    const int64_t most = (c.units + 4 * kThreads - 1) / (4 * kThreads);
+    const int64_t want = (148 * 8 + pages - 1) / pages;
+    const int64_t parts = want < most ? want : most, part = (c.units + parts - 1) / parts;
+    page_copy_kernel<V><<<grid_for(pages * parts, 1), kThreads, 0, s>>>(c, (int)parts, part);
+  }
+  return check_launch("page_copy");
 }
 
 }  // namespace
@@ -675,23 +798,20 @@ int tg_paged_append(int dtype, int64_t batch, int64_t tokens, int64_t kv_heads, 
   cudaStream_t s = as_stream(stream);
   return TG_DISPATCH_FLOAT(dtype, T, [&] {
     constexpr int64_t U = 16 / sizeof(T);
+    Moves m;
     const Pool p{num_pages, kv_heads, page_size, head_dim, pages, max_pages, bad_page_dev};
+    const int r = make_moves("paged_append", p, batch, tokens, lengths, m);
+    if (r) return r;
     const int64_t strides = k_sb | k_sh | k_st | v_sb | v_sh | v_st;
-    const int64_t total = batch * tokens * kv_heads * head_dim;
     if (head_dim % U == 0 && strides % U == 0 && aligned16(k) && aligned16(v) &&
         aligned16(key_pages) && aligned16(value_pages)) {
-      Pool pu = p;
-      pu.head_dim /= U;
-      append_kernel<Unit16><<<grid_for(total / U, kThreads), kThreads, 0, s>>>(
-          pu, batch, tokens, (const Unit16*)k, Rows{k_sb / U, k_sh / U, k_st / U},
-          (const Unit16*)v, Rows{v_sb / U, v_sh / U, v_st / U}, lengths, (Unit16*)key_pages,
-          (Unit16*)value_pages);
-    } else {
-      append_kernel<T><<<grid_for(total, kThreads), kThreads, 0, s>>>(
-          p, batch, tokens, (const T*)k, Rows{k_sb, k_sh, k_st}, (const T*)v,
-          Rows{v_sb, v_sh, v_st}, lengths, (T*)key_pages, (T*)value_pages);
+      m.pool.head_dim /= U;
+      return launch_append(m, (const Unit16*)k, Rows{k_sb / U, k_sh / U, k_st / U},
+                           (const Unit16*)v, Rows{v_sb / U, v_sh / U, v_st / U},
+                           (Unit16*)key_pages, (Unit16*)value_pages, s);
     }
-    return check_launch("paged_append");
+    return launch_append(m, (const T*)k, Rows{k_sb, k_sh, k_st}, (const T*)v,
+                         Rows{v_sb, v_sh, v_st}, (T*)key_pages, (T*)value_pages, s);
   });
 }
 
@@ -706,20 +826,17 @@ int tg_paged_gather(int dtype, int64_t batch, int64_t longest, int64_t kv_heads,
   cudaStream_t s = as_stream(stream);
   return TG_DISPATCH_FLOAT(dtype, T, [&] {
     constexpr int64_t U = 16 / sizeof(T);
+    Moves m;
     const Pool p{num_pages, kv_heads, page_size, head_dim, pages, max_pages, bad_page_dev};
-    const int64_t total = batch * longest * kv_heads * head_dim;
+    const int r = make_moves("paged_gather", p, batch, longest, lengths, m);
+    if (r) return r;
     if (head_dim % U == 0 && aligned16(k) && aligned16(v) && aligned16(key_pages) &&
         aligned16(value_pages)) {
-      Pool pu = p;
-      pu.head_dim /= U;
-      gather_kernel<Unit16><<<grid_for(total / U, kThreads), kThreads, 0, s>>>(
-          pu, batch, longest, (const Unit16*)key_pages, (const Unit16*)value_pages, lengths,
-          (Unit16*)k, (Unit16*)v);
-    } else {
-      gather_kernel<T><<<grid_for(total, kThreads), kThreads, 0, s>>>(
-          p, batch, longest, (const T*)key_pages, (const T*)value_pages, lengths, (T*)k, (T*)v);
+      m.pool.head_dim /= U;
+      return launch_gather(m, (const Unit16*)key_pages, (const Unit16*)value_pages, (Unit16*)k,
+                           (Unit16*)v, s);
     }
-    return check_launch("paged_gather");
+    return launch_gather(m, (const T*)key_pages, (const T*)value_pages, (T*)k, (T*)v, s);
   });
 }
 
@@ -730,16 +847,13 @@ int tg_page_copy(int64_t page_bytes, int64_t layers, int64_t num_pages, void* ke
                "page_copy: bad sizes");
   if (pairs == 0) return TG_OK;
   cudaStream_t s = as_stream(stream);
-  const unsigned grid = grid_for(2 * layers * pairs, 1);
   if (page_bytes % 16 == 0 && aligned16(key_pages) && aligned16(value_pages))
-    page_copy_kernel<Unit16><<<grid, kThreads, 0, s>>>(
-        (Unit16*)key_pages, (Unit16*)value_pages, layers, num_pages, page_bytes / 16, src, dst,
-        pairs, bad_page_dev);
-  else
-    page_copy_kernel<uint32_t><<<grid, kThreads, 0, s>>>(
-        (uint32_t*)key_pages, (uint32_t*)value_pages, layers, num_pages, page_bytes / 4, src, dst,
-        pairs, bad_page_dev);
-  return check_launch("page_copy");
+    return launch_copies(Copies<Unit16>{(Unit16*)key_pages, (Unit16*)value_pages, layers,
+                                        num_pages, page_bytes / 16, src, dst, pairs,
+                                        bad_page_dev}, s);
+  return launch_copies(Copies<uint32_t>{(uint32_t*)key_pages, (uint32_t*)value_pages, layers,
+                                        num_pages, page_bytes / 4, src, dst, pairs,
+                                        bad_page_dev}, s);
 }
 
 size_t tg_paged_attention_scratch_bytes(int dtype, int64_t batch, int64_t heads, int64_t kv_heads,
@@ -762,9 +876,6 @@ int tg_paged_attention(int dtype, int64_t batch, int64_t heads, int64_t kv_heads
   TG_CHECK_ARG(batch >= 0 && heads > 0 && heads % kv_heads == 0,
                "paged_attention: %lld query heads over %lld key heads", (long long)heads,
                (long long)kv_heads);
-  TG_CHECK_ARG(num_pages <= INT32_MAX && max_pages <= (INT32_MAX - (1 << 16)) / page_size,
-               "paged_attention: positions up to 2^31 (table of %lld pages of %lld)",
-               (long long)max_pages, (long long)page_size);
   if (head_dim > kMaxHead)
     return set_error(TG_ERR_UNSUPPORTED, "paged_attention: head_dim %lld (at most %d)",
                      (long long)head_dim, kMaxHead);

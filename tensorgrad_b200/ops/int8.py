@@ -133,8 +133,10 @@ def int8_linear(x: Any, weight: Int8Weight, bias: Any = None) -> Tensor:
         b = tb.data if tb.dtype == x_.dtype else cast_array(tb.data, x_.dtype)
     rows = x_.size // inner
     y = device.empty((*tx.shape[:-1], outer), x_.dtype)
-    scratch = device.scratch(lib.tg_int8_linear_scratch_bytes(code, rows, inner, outer))
+    nbytes = lib.tg_int8_linear_scratch_bytes(code, rows, inner, outer)
+    scratch = device.scratch(nbytes) if nbytes > 16 else None
     check(lib.tg_int8_linear(code, x_.ptr, rows, inner, weight.q.ptr, weight.q.shape[1],
-                             scale.ptr, None if b is None else b.ptr, y.ptr, outer, scratch.ptr,
-                             device.stream()), "int8_linear")
+                             scale.ptr, None if b is None else b.ptr, y.ptr, outer,
+                             None if scratch is None else scratch.ptr, device.stream()),
+          "int8_linear")
     return Tensor._wrap(y)

@@ -257,9 +257,10 @@ def token_log_probs(logits: Any, targets: Any, *, top_k: int = 0,
     if tl.ndim == 0 or tl.shape[-1] == 0:
         raise ValueError(f"token_log_probs needs a class axis, got logits {tl.shape}")
     lead, classes = tl.shape[:-1], tl.shape[-1]
-    most = min(int(lib.tg_token_log_probs_max_top()), classes)
-    if not 0 <= top_k <= most:
-        raise ValueError(f"top_k must be in [0, {most}] for {classes} classes, got {top_k}")
+    if top_k != 0:
+        most = min(int(lib.tg_token_log_probs_max_top()), classes)
+        if not 0 <= top_k <= most:
+            raise ValueError(f"top_k must be in [0, {most}] for {classes} classes, got {top_k}")
     tgt, bad = _class_targets("token_log_probs", tl, targets, ignore_index)
     x = tl.data if tl.dtype.kind == "f" else cast_array(tl.data, np.dtype(np.float64))
     rows = math.prod(lead)
