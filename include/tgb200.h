@@ -338,7 +338,8 @@ int tg_token_log_probs_forward(int dtype, const void* logits, const int64_t* tar
                                int64_t* top_ids, int64_t rows, int64_t classes, int64_t top_k,
                                int64_t ignore_index, int* bad_target_dev, void* stream);
 /* grad[row][j] = g_log[row] [j == t] + sum_k g_top[row][k] [j == top_ids[row][k]]
- *   - p_j (g_log[row] + sum_k g_top[row][k] + g_ent[row] (log p_j + entropy[row])). */
+ *   - p_j (g_log[row] + sum_k g_top[row][k] + g_ent[row] (log p_j + entropy[row])).
+ * g_log, g_ent and g_top may each be NULL: no gradient comes in there. */
 int tg_token_log_probs_backward(int dtype, const void* logits, const int64_t* targets,
                                 const void* stats, const void* entropy, const int64_t* top_ids,
                                 const void* g_log, const void* g_ent, const void* g_top,

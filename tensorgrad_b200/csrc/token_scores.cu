@@ -369,7 +369,7 @@ scores_bwd_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targ
     const T inv = T(1) / s, ls = dev_log<T>(s);
     const int64_t t = targets[r];
     const bool given = t != ignore_index && t >= 0 && t < classes;
-    const T gl = given ? g_log[r] : T(0), ge = g_ent[r];
+    const T gl = given && g_log ? g_log[r] : T(0), ge = g_ent ? g_ent[r] : T(0);
     T tops = T(0);
     for (int k = threadIdx.x & 31; k < top_k; k += 32) tops += g_top[r * top_k + k];
     if (top_k > 0) tops = warp_sum(tops);
@@ -484,6 +484,7 @@ int tg_token_log_probs_backward(int dtype, const void* logits, const int64_t* ta
   cudaStream_t s = as_stream(stream);
   return TG_DISPATCH_FLOAT(dtype, T, [&] {
     constexpr int VE = 16 / sizeof(T);
+    if (!g_top) top_k = 0;  // no gradient comes in through the alternatives
     const int parts = row_splits(rows, classes);
     const int part = (int)((classes + parts * VE - 1) / (parts * VE) * VE);
     const int64_t most = (int64_t)sm_count() * 8;

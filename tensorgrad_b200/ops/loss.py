@@ -220,16 +220,37 @@ def _class_targets(what: str, tl: Tensor, target: Any,
     return device.from_numpy(flat), None
 
 
-def _part(packed: Tensor, offset: int, shape: tuple[int, ...]) -> Tensor:
-    """A contiguous part of a packed result as a view; its VJP puts the gradient into zeros
-    of the packed size."""
-    total = packed.size
-    count = math.prod(shape)
+class _PartGradients:
+    """The gradient of a packed result as the gradients of its parts, by their offsets: the
+    engine's sum over the parts' VJPs joins them without device work."""
 
-    def backward(g: DeviceArray, need: Need) -> tuple[DeviceArray]:
-        out = device.zeros((total,), g.dtype)
-        device.copy_into(out.flat_view(offset, count), g)
-        return (out,)
+    __slots__ = ("parts", "shape")
+
+    def __init__(self, shape: tuple[int, ...], parts: dict[int, DeviceArray]) -> None:
+        self.shape, self.parts = shape, parts
+
+    def __add__(self, other: _PartGradients) -> _PartGradients:
+        parts = dict(self.parts)
+        for offset, g in other.parts.items():
+            parts[offset] = parts[offset] + g if offset in parts else g
+        return _PartGradients(self.shape, parts)
+
+    def pointer(self, offset: int, dtype: np.dtype[Any], keep: list[DeviceArray]) -> int | None:
+        """Address of a part's gradient in ``dtype`` (kept alive in ``keep``), None without one."""
+        g = self.parts.get(offset)
+        if g is None:
+            return None
+        keep.append(g if g.dtype == dtype else cast_array(g, dtype))
+        return keep[-1].ptr
+
+
+def _part(packed: Tensor, offset: int, shape: tuple[int, ...]) -> Tensor:
+    """A contiguous part of a packed result as a view. Its VJP hands the gradient on as that
+    part's; the graph VJP puts it into zeros of the packed size."""
+    total, count = packed.size, math.prod(shape)
+
+    def backward(g: DeviceArray, need: Need) -> tuple[Any]:
+        return (_PartGradients((total,), {offset: g}),)
 
     def graph(g: Tensor, y: Tensor, need: Need) -> tuple[Tensor]:
         from tensorgrad_b200.ops.shape import _scatter, reshape
@@ -284,14 +305,15 @@ def token_log_probs(logits: Any, targets: Any, *, top_k: int = 0,
             None if ids is None else
             Tensor._wrap(whole.flat_view(2 * rows, rows * top_k, ids.shape)), top_ids)
 
-    def backward(g: DeviceArray, need: Need) -> tuple[DeviceArray]:
-        if g.dtype != x.dtype:
-            g = cast_array(g, x.dtype)
+    def backward(g: Any, need: Need) -> tuple[DeviceArray]:
+        # Only the parts' VJPs reach this node.
+        keep: list[DeviceArray] = []
+        given = [g.pointer(at, x.dtype, keep) for at in (0, rows, 2 * rows)]
         grad = device.empty(tl.shape, x.dtype)
         check(lib.tg_token_log_probs_backward(
-            code, x.ptr, tgt.ptr, whole.ptr + size * es, whole.ptr + rows * es, ids_ptr, g.ptr,
-            g.ptr + rows * es, g.ptr + 2 * rows * es, grad.ptr, rows, classes, top_k,
-            ignore_index, device.stream()), "token_log_probs backward")
+            code, x.ptr, tgt.ptr, whole.ptr + size * es, whole.ptr + rows * es, ids_ptr, *given,
+            grad.ptr, rows, classes, top_k, ignore_index, device.stream()),
+            "token_log_probs backward")
         return (grad if grad.dtype == tl.dtype else cast_array(grad, tl.dtype),)
 
     def graph(g: Tensor, y: Tensor, need: Need) -> tuple[Tensor | None, ...]:

@@ -217,6 +217,33 @@ def test_gradients_against_differences():
     gradgradcheck(total, [x])
 
 
+def test_each_output_alone_and_used_twice():
+    import tensorgrad_b200 as tg
+
+    rng = np.random.default_rng(12)
+    x = rng.standard_normal((4, 9))
+    t = np.array([3, -100, 0, 8])
+    g = [rng.standard_normal(4), rng.standard_normal(4), rng.standard_normal((4, 3))]
+
+    def grads(wanted, times=1):
+        tx = tg.Tensor(x, requires_grad=True)
+        got = tg.token_log_probs(tx, t, top_k=3)
+        outs = [got.log_probs, got.entropy, got.top_log_probs]
+        total = None
+        for i in wanted:
+            for _ in range(times):
+                term = (outs[i] * tg.Tensor(g[i] / times)).sum()
+                total = term if total is None else total + term
+        total.backward()
+        return tx.grad.numpy()
+
+    one = [grads([i]) for i in range(3)]
+    np.testing.assert_allclose(grads([0, 1, 2]), sum(one), rtol=0, atol=1e-14)
+    np.testing.assert_allclose(grads([2, 0]), one[0] + one[2], rtol=0, atol=1e-14)
+    for i in range(3):
+        np.testing.assert_allclose(grads([i], times=2), one[i], rtol=0, atol=1e-14)
+
+
 def test_matches_cross_entropy_through_the_model_path():
     import tensorgrad_b200 as tg
 
