@@ -261,7 +261,6 @@ struct ScoreArgs {
   T* entropy;
   T* top;
   int64_t* ids;
-  int64_t rows;
   int classes, top_k, splits, part;  // part: classes of a split, a multiple of VE
   int64_t ignore_index;
   int* bad_target;
@@ -278,74 +277,72 @@ scores_fwd_kernel(ScoreArgs<T> a) {
   pdl_trigger();
   pdl_wait();
   const int split = blockIdx.x % a.splits;
-  for (int64_t r = blockIdx.x / a.splits; r < a.rows; r += gridDim.x / a.splits) {
-    const int first = split * a.part;
-    const int n = a.classes - first < a.part ? a.classes - first : a.part;
-    const T* row = a.logits + r * a.classes;
-    const T* x = row + first;
-    Stats<T> mine{kLowest<T>, T(0), T(0)};
-    const int units = n / VE;  // parts are multiples of VE
-    const Vec<T, VE>* xv = reinterpret_cast<const Vec<T, VE>*>(x);
-    int c = threadIdx.x;
+  const int64_t r = blockIdx.x / a.splits;
+  const int first = split * a.part;
+  const int n = a.classes - first < a.part ? a.classes - first : a.part;
+  const T* row = a.logits + r * a.classes;
+  const T* x = row + first;
+  Stats<T> mine{kLowest<T>, T(0), T(0)};
+  const int units = n / VE;  // parts are multiples of VE
+  const Vec<T, VE>* xv = reinterpret_cast<const Vec<T, VE>*>(x);
+  int c = threadIdx.x;
 #pragma unroll 1
-    for (; c + (N - 1) * kThreads < units; c += N * kThreads) {
-      T v[N * VE];
+  for (; c + (N - 1) * kThreads < units; c += N * kThreads) {
+    T v[N * VE];
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const Vec<T, VE> y = xv[c + i * kThreads];
+    for (int i = 0; i < N; ++i) {
+      const Vec<T, VE> y = xv[c + i * kThreads];
 #pragma unroll
-        for (int e = 0; e < VE; ++e) v[i * VE + e] = y.v[e];
+      for (int e = 0; e < VE; ++e) v[i * VE + e] = y.v[e];
+    }
+    push(mine, v);
+  }
+  for (; c < units; c += kThreads) {
+    const Vec<T, VE> y = xv[c];
+    push(mine, y.v);
+  }
+  const T lane_top = mine.m;
+  mine = block_join(mine, sh.stats);
+  if (a.top_k > 0) select_top<T, VE>(x, n, first, a.top_k, lane_top, sh);
+  if (a.splits > 1) {
+    const auto cluster = cooperative_groups::this_cluster();
+    if (threadIdx.x == 0) sh.mine = mine;
+    cluster.sync();
+    const int other = threadIdx.x & 7;
+    mine = lanes_join<8>(other < a.splits ? *cluster.map_shared_rank(&sh.mine, other)
+                                          : Stats<T>{kLowest<T>, T(0), T(0)});
+    if (split == 0) {
+      for (int i = threadIdx.x; i < a.splits * a.top_k; i += kThreads)
+        sh.list[i] = cluster.map_shared_rank(sh.best, i / a.top_k)[i % a.top_k];
+    }
+    cluster.sync();  // the others' results have been read
+  }
+  if (split != 0) return;
+  const T ls = dev_log<T>(mine.s);
+  const T m = mine.s != T(0) ? mine.m : T(-INFINITY);  // a closed row has no log probabilities
+  auto place = [&](int rank, Alt<U> e) {
+    a.top[r * a.top_k + rank] = (row[e.id] - m) - ls;
+    a.ids[r * a.top_k + rank] = e.id;
+  };
+  if (a.splits > 1) {
+    rank_list(a.splits * a.top_k, a.top_k, sh, place);
+  } else {
+    for (int k = threadIdx.x; k < a.top_k; k += kThreads) place(k, sh.best[k]);
+  }
+  if (threadIdx.x == 0) {
+    a.stats[2 * r] = m;
+    a.stats[2 * r + 1] = mine.s;
+    a.entropy[r] = ls - mine.u / mine.s;
+    const int64_t t = a.targets[r];
+    T lp = T(0);
+    if (t != a.ignore_index) {
+      if (t < 0 || t >= a.classes) {
+        if (a.bad_target) *a.bad_target = 1;
+      } else {
+        lp = (row[t] - m) - ls;
       }
-      push(mine, v);
     }
-    for (; c < units; c += kThreads) {
-      const Vec<T, VE> y = xv[c];
-      push(mine, y.v);
-    }
-    const T lane_top = mine.m;
-    mine = block_join(mine, sh.stats);
-    if (a.top_k > 0) select_top<T, VE>(x, n, first, a.top_k, lane_top, sh);
-    if (a.splits > 1) {
-      const auto cluster = cooperative_groups::this_cluster();
-      if (threadIdx.x == 0) sh.mine = mine;
-      cluster.sync();
-      const int other = threadIdx.x & 7;
-      mine = lanes_join<8>(other < a.splits ? *cluster.map_shared_rank(&sh.mine, other)
-                                            : Stats<T>{kLowest<T>, T(0), T(0)});
-      if (split == 0) {
-        for (int i = threadIdx.x; i < a.splits * a.top_k; i += kThreads)
-          sh.list[i] = cluster.map_shared_rank(sh.best, i / a.top_k)[i % a.top_k];
-      }
-      cluster.sync();  // the others' results have been read
-    }
-    if (split != 0) continue;
-    const T ls = dev_log<T>(mine.s);
-    const T m = mine.s != T(0) ? mine.m : T(-INFINITY);  // a closed row has no log probabilities
-    auto place = [&](int rank, Alt<U> e) {
-      a.top[r * a.top_k + rank] = (row[e.id] - m) - ls;
-      a.ids[r * a.top_k + rank] = e.id;
-    };
-    if (a.splits > 1) {
-      rank_list(a.splits * a.top_k, a.top_k, sh, place);
-    } else {
-      for (int k = threadIdx.x; k < a.top_k; k += kThreads) place(k, sh.best[k]);
-    }
-    if (threadIdx.x == 0) {
-      a.stats[2 * r] = m;
-      a.stats[2 * r + 1] = mine.s;
-      a.entropy[r] = ls - mine.u / mine.s;
-      const int64_t t = a.targets[r];
-      T lp = T(0);
-      if (t != a.ignore_index) {
-        if (t < 0 || t >= a.classes) {
-          if (a.bad_target) *a.bad_target = 1;
-        } else {
-          lp = (row[t] - m) - ls;
-        }
-      }
-      a.log_probs[r] = lp;
-    }
-    __syncthreads();
+    a.log_probs[r] = lp;
   }
 }
 
@@ -357,53 +354,52 @@ scores_bwd_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targ
                   const T* __restrict__ stats, const T* __restrict__ entropy,
                   const int64_t* __restrict__ ids, const T* __restrict__ g_log,
                   const T* __restrict__ g_ent, const T* __restrict__ g_top, T* __restrict__ grad,
-                  int64_t rows, int classes, int part, int top_k, int64_t ignore_index) {
+                  int classes, int part, int top_k, int64_t ignore_index) {
   pdl_trigger();
   pdl_wait();
   const int first = blockIdx.y * part;
   const int n = classes - first < part ? classes - first : part;
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const T* x = logits + r * classes + first;
-    T* d = grad + r * classes + first;
-    const T m = stats[2 * r], s = stats[2 * r + 1];
-    const T inv = T(1) / s, ls = dev_log<T>(s);
-    const int64_t t = targets[r];
-    const bool given = t != ignore_index && t >= 0 && t < classes;
-    const T gl = given && g_log ? g_log[r] : T(0), ge = g_ent ? g_ent[r] : T(0);
-    T tops = T(0);
-    for (int k = threadIdx.x & 31; k < top_k; k += 32) tops += g_top[r * top_k + k];
-    if (top_k > 0) tops = warp_sum(tops);
-    // -p (a + ge z) with z = x - m: log p + H = z + (H - log s).
-    const T a = gl + tops + ge * (entropy[r] - ls);
-    auto one = [&](T v) {
-      const T z = v - m, p = exp_below(z) * inv;
-      return p == T(0) ? T(0) : -p * (a + ge * z);  // nothing is left where log p may be -inf
-    };
-    const int units = n / VE;
-    const Vec<T, VE>* xv = reinterpret_cast<const Vec<T, VE>*>(x);
-    Vec<T, VE>* dv = reinterpret_cast<Vec<T, VE>*>(d);
+  const int64_t r = blockIdx.x;
+  const T* x = logits + r * classes + first;
+  T* d = grad + r * classes + first;
+  const T m = stats[2 * r], s = stats[2 * r + 1];
+  const T inv = T(1) / s, ls = dev_log<T>(s);
+  const int64_t t = targets[r];
+  const bool given = t != ignore_index && t >= 0 && t < classes;
+  const T gl = given && g_log ? g_log[r] : T(0), ge = g_ent ? g_ent[r] : T(0);
+  T tops = T(0);
+  for (int k = threadIdx.x & 31; k < top_k; k += 32) tops += g_top[r * top_k + k];
+  if (top_k > 0) tops = warp_sum(tops);
+  // -p (a + ge z) with z = x - m: log p + H = z + (H - log s).
+  const T a = gl + tops + ge * (entropy[r] - ls);
+  auto one = [&](T v) {
+    const T z = v - m, p = exp_below(z) * inv;
+    return p == T(0) ? T(0) : -p * (a + ge * z);  // nothing is left where log p may be -inf
+  };
+  const int units = n / VE;
+  const Vec<T, VE>* xv = reinterpret_cast<const Vec<T, VE>*>(x);
+  Vec<T, VE>* dv = reinterpret_cast<Vec<T, VE>*>(d);
 #pragma unroll 4
-    for (int c = threadIdx.x; c < units; c += kThreads) {
-      Vec<T, VE> v = xv[c];
+  for (int c = threadIdx.x; c < units; c += kThreads) {
+    Vec<T, VE> v = xv[c];
 #pragma unroll
-      for (int e = 0; e < VE; ++e) v.v[e] = one(v.v[e]);
-      dv[c] = v;
-    }
-    // The single classes, by one lane each: the alternatives are distinct, the target may be
-    // one of them.
-    bool hit = false;
-    const int64_t at = t - first;
-    __syncthreads();
-    for (int k = threadIdx.x; k < top_k; k += kThreads) {
-      const int64_t i = ids[r * top_k + k] - first;
-      if (i < 0 || i >= n) continue;
-      const bool same = given && i == at;
-      hit |= same;
-      d[i] += g_top[r * top_k + k] + (same ? gl : T(0));
-    }
-    hit = __syncthreads_or(hit);
-    if (threadIdx.x == 0 && given && !hit && at >= 0 && at < n) d[at] += gl;
+    for (int e = 0; e < VE; ++e) v.v[e] = one(v.v[e]);
+    dv[c] = v;
   }
+  // The single classes, by one lane each: the alternatives are distinct, the target may be
+  // one of them.
+  bool hit = false;
+  const int64_t at = t - first;
+  __syncthreads();
+  for (int k = threadIdx.x; k < top_k; k += kThreads) {
+    const int64_t i = ids[r * top_k + k] - first;
+    if (i < 0 || i >= n) continue;
+    const bool same = given && i == at;
+    hit |= same;
+    d[i] += g_top[r * top_k + k] + (same ? gl : T(0));
+  }
+  hit = __syncthreads_or(hit);
+  if (threadIdx.x == 0 && given && !hit && at >= 0 && at < n) d[at] += gl;
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -440,7 +436,8 @@ int tg_token_log_probs_forward(int dtype, const void* logits, const int64_t* tar
                                void* log_probs, void* entropy, void* top_log_probs,
                                int64_t* top_ids, int64_t rows, int64_t classes, int64_t top_k,
                                int64_t ignore_index, int* bad_target_dev, void* stream) {
-  TG_CHECK_ARG(rows >= 0 && classes > 0 && classes <= kMaxClasses, "token_log_probs: bad shape");
+  TG_CHECK_ARG(rows >= 0 && rows <= INT32_MAX && classes > 0 && classes <= kMaxClasses,
+               "token_log_probs: bad shape");
   TG_CHECK_ARG(top_k >= 0 && top_k <= kMaxTop && top_k <= classes,
                "token_log_probs: top_k %lld (at most %d and the %lld classes)", (long long)top_k,
                kMaxTop, (long long)classes);
@@ -450,13 +447,12 @@ int tg_token_log_probs_forward(int dtype, const void* logits, const int64_t* tar
   return TG_DISPATCH_FLOAT(dtype, T, [&] {
     constexpr int VE = 16 / sizeof(T);
     ScoreArgs<T> a{(const T*)logits, targets, (T*)stats, (T*)log_probs, (T*)entropy,
-                   (T*)top_log_probs, top_ids, rows, (int)classes, (int)top_k, 1, (int)classes,
+                   (T*)top_log_probs, top_ids, (int)classes, (int)top_k, 1, (int)classes,
                    ignore_index, bad_target_dev};
     a.splits = row_splits(rows, classes);
     if (a.splits > 1) a.part = (int)((classes + a.splits * VE - 1) / (a.splits * VE) * VE);
-    const int64_t most = (int64_t)sm_count() * 8;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((rows < most ? rows : most) * a.splits));
+    cfg.gridDim = dim3((unsigned)(rows * a.splits));
     cfg.blockDim = dim3(kThreads);
     cfg.stream = s;
     cudaLaunchAttribute at[2];
@@ -478,8 +474,8 @@ int tg_token_log_probs_backward(int dtype, const void* logits, const int64_t* ta
                                 const void* g_log, const void* g_ent, const void* g_top,
                                 void* grad, int64_t rows, int64_t classes, int64_t top_k,
                                 int64_t ignore_index, void* stream) {
-  TG_CHECK_ARG(rows >= 0 && classes > 0 && classes <= kMaxClasses && top_k >= 0 &&
-                   top_k <= kMaxTop, "token_log_probs backward: bad shape");
+  TG_CHECK_ARG(rows >= 0 && rows <= INT32_MAX && classes > 0 && classes <= kMaxClasses &&
+                   top_k >= 0 && top_k <= kMaxTop, "token_log_probs backward: bad shape");
   if (rows == 0) return TG_OK;
   cudaStream_t s = as_stream(stream);
   return TG_DISPATCH_FLOAT(dtype, T, [&] {
@@ -487,13 +483,12 @@ int tg_token_log_probs_backward(int dtype, const void* logits, const int64_t* ta
     if (!g_top) top_k = 0;  // no gradient comes in through the alternatives
     const int parts = row_splits(rows, classes);
     const int part = (int)((classes + parts * VE - 1) / (parts * VE) * VE);
-    const int64_t most = (int64_t)sm_count() * 8;
-    const dim3 grid((unsigned)(rows < most ? rows : most), (unsigned)parts);
+    const dim3 grid((unsigned)rows, (unsigned)parts);
     const bool vec = classes % VE == 0 && aligned16(logits) && aligned16(grad);
     TG_CUDA_TRY(launch_pdl(vec ? scores_bwd_kernel<T, VE> : scores_bwd_kernel<T, 1>, grid,
                            dim3(kThreads), 0, s, (const T*)logits, targets, (const T*)stats,
                            (const T*)entropy, top_ids, (const T*)g_log, (const T*)g_ent,
-                           (const T*)g_top, (T*)grad, rows, (int)classes, part, (int)top_k,
+                           (const T*)g_top, (T*)grad, (int)classes, part, (int)top_k,
                            ignore_index));
     return check_launch("token_log_probs backward");
   });
