@@ -266,6 +266,46 @@ struct ScoreArgs {
   int* bad_target;
 };
 
+// The target's log probability; 0 without one.
+template <typename T>
+__device__ __forceinline__ T target_log_prob(const ScoreArgs<T>& a, int64_t r, const T* row, T m,
+                                             T ls) {
+  const int64_t t = a.targets[r];
+  if (t == a.ignore_index) return T(0);
+  if (t < 0 || t >= a.classes) {
+    if (a.bad_target) *a.bad_target = 1;
+    return T(0);
+  }
+  return (row[t] - m) - ls;
+}
+
+// A row's part of the VJP: dx_j = -p_j (g_log + sum g_top + g_ent (log p_j + H)), then g_log at the
+// target and g_top at the alternatives. Built by whole warps.
+template <typename T>
+struct Pull {
+  T m, inv, a, slope, log;  // -p (a + slope z) with z = x - m: log p + H = z + (H - log s)
+  int64_t target;           // -1 without one
+  __device__ Pull(int64_t r, int classes, const int64_t* targets, const T* stats,
+                  const T* entropy, const T* g_log, const T* g_ent, const T* g_top, int top_k,
+                  int64_t ignore_index) {
+    m = stats[2 * r];
+    const T s = stats[2 * r + 1], ls = dev_log<T>(s);
+    inv = T(1) / s;
+    target = targets[r];
+    if (target == ignore_index || target < 0 || target >= classes) target = -1;
+    log = target >= 0 && g_log ? g_log[r] : T(0);
+    slope = g_ent ? g_ent[r] : T(0);
+    T tops = T(0);
+    for (int k = threadIdx.x & 31; k < top_k; k += 32) tops += g_top[r * top_k + k];
+    if (top_k > 0) tops = warp_sum(tops);
+    a = log + tops + slope * (entropy[r] - ls);
+  }
+  __device__ __forceinline__ T spread(T x) const {
+    const T z = x - m, p = exp_below(z) * inv;
+    return p == T(0) ? T(0) : -p * (a + slope * z);  // nothing is left where log p may be -inf
+  }
+};
+
 // One block a row, or a cluster of `splits` blocks with a part of its classes each. HBM-bound: one
 // read of the logits, VE of them to a load; 8 instructions and one exponential a value.
 template <typename T, int VE>
@@ -333,21 +373,11 @@ scores_fwd_kernel(ScoreArgs<T> a) {
     a.stats[2 * r] = m;
     a.stats[2 * r + 1] = mine.s;
     a.entropy[r] = ls - mine.u / mine.s;
-    const int64_t t = a.targets[r];
-    T lp = T(0);
-    if (t != a.ignore_index) {
-      if (t < 0 || t >= a.classes) {
-        if (a.bad_target) *a.bad_target = 1;
-      } else {
-        lp = (row[t] - m) - ls;
-      }
-    }
-    a.log_probs[r] = lp;
+    a.log_probs[r] = target_log_prob(a, r, row, m, ls);
   }
 }
 
-// dx_j = -p_j (g_log + sum g_top + g_ent (log p_j + H)), then g_log at the target and g_top at
-// the alternatives. Block (row, part of the classes); one read of the logits, one write.
+// Block (row, part of the classes); one read of the logits, one write.
 template <typename T, int VE>
 __global__ void __launch_bounds__(kThreads)
 scores_bwd_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targets,
@@ -360,46 +390,130 @@ scores_bwd_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targ
   const int first = blockIdx.y * part;
   const int n = classes - first < part ? classes - first : part;
   const int64_t r = blockIdx.x;
-  const T* x = logits + r * classes + first;
+  const Pull<T> p(r, classes, targets, stats, entropy, g_log, g_ent, g_top, top_k, ignore_index);
   T* d = grad + r * classes + first;
-  const T m = stats[2 * r], s = stats[2 * r + 1];
-  const T inv = T(1) / s, ls = dev_log<T>(s);
-  const int64_t t = targets[r];
-  const bool given = t != ignore_index && t >= 0 && t < classes;
-  const T gl = given && g_log ? g_log[r] : T(0), ge = g_ent ? g_ent[r] : T(0);
-  T tops = T(0);
-  for (int k = threadIdx.x & 31; k < top_k; k += 32) tops += g_top[r * top_k + k];
-  if (top_k > 0) tops = warp_sum(tops);
-  // -p (a + ge z) with z = x - m: log p + H = z + (H - log s).
-  const T a = gl + tops + ge * (entropy[r] - ls);
-  auto one = [&](T v) {
-    const T z = v - m, p = exp_below(z) * inv;
-    return p == T(0) ? T(0) : -p * (a + ge * z);  // nothing is left where log p may be -inf
-  };
   const int units = n / VE;
-  const Vec<T, VE>* xv = reinterpret_cast<const Vec<T, VE>*>(x);
+  const Vec<T, VE>* xv = reinterpret_cast<const Vec<T, VE>*>(logits + r * classes + first);
   Vec<T, VE>* dv = reinterpret_cast<Vec<T, VE>*>(d);
 #pragma unroll 4
   for (int c = threadIdx.x; c < units; c += kThreads) {
     Vec<T, VE> v = xv[c];
 #pragma unroll
-    for (int e = 0; e < VE; ++e) v.v[e] = one(v.v[e]);
+    for (int e = 0; e < VE; ++e) v.v[e] = p.spread(v.v[e]);
     dv[c] = v;
   }
   // The single classes, by one lane each: the alternatives are distinct, the target may be
   // one of them.
   bool hit = false;
-  const int64_t at = t - first;
+  const int64_t at = p.target - first;
   __syncthreads();
   for (int k = threadIdx.x; k < top_k; k += kThreads) {
     const int64_t i = ids[r * top_k + k] - first;
     if (i < 0 || i >= n) continue;
-    const bool same = given && i == at;
+    const bool same = p.target >= 0 && i == at;
     hit |= same;
-    d[i] += g_top[r * top_k + k] + (same ? gl : T(0));
+    d[i] += g_top[r * top_k + k] + (same ? p.log : T(0));
   }
   hit = __syncthreads_or(hit);
-  if (threadIdx.x == 0 && given && !hit && at >= 0 && at < n) d[at] += gl;
+  if (threadIdx.x == 0 && p.target >= 0 && !hit && at >= 0 && at < n) d[at] += p.log;
+}
+
+// Rows of up to kWarpRow classes: a warp a row, its values in registers (NV of them to a lane),
+// alternatives taken one by one. A block a row leaves most of its lanes idle there (8192 rows of 65
+// classes forward and backward: 42.5 us, with a warp a row 7.1).
+constexpr int kWarpRow = 1024;
+
+template <typename T, int NV>
+__global__ void __launch_bounds__(kThreads)
+scores_fwd_warp_kernel(ScoreArgs<T> a, int64_t rows) {
+  using U = typename OrderKey<T>::U;
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  const T* row = a.logits + r * a.classes;
+  T v[NV], m = kLowest<T>, s = T(0), u = T(0);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = lane + 32 * i;
+    v[i] = c < a.classes ? row[c] : T(-INFINITY);
+    m = fmax(m, v[i]);
+  }
+  m = warp_max(m);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const T z = v[i] - m, e = exp_below(z);
+    s += e;
+    u += e * fmax(z, kLowest<T>);
+  }
+  s = warp_sum(s);
+  u = warp_sum(u);
+  const T ls = dev_log<T>(s);
+  if (s == T(0)) m = T(-INFINITY);  // a closed row has no log probabilities
+  if (a.top_k > 0) {
+    // Every lane offers its first entry that has not been taken; the one that wins looks for
+    // its next.
+    uint32_t taken = 0;
+    Alt<U> mine;
+    auto offer = [&] {
+      mine = {0, std::numeric_limits<int>::max()};
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = lane + 32 * i;
+        const Alt<U> e{OrderKey<T>::of(v[i]), c};
+        if (c < a.classes && !(taken >> i & 1) && before(e, mine)) mine = e;
+      }
+    };
+    offer();
+    for (int k = 0; k < a.top_k; ++k) {
+      Alt<U> best = mine;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const Alt<U> other{__shfl_xor_sync(0xffffffffu, best.key, o),
+                           __shfl_xor_sync(0xffffffffu, best.id, o)};
+        if (before(other, best)) best = other;
+      }
+      if (best.id % 32 == lane) {
+        a.top[r * a.top_k + k] = (row[best.id] - m) - ls;
+        a.ids[r * a.top_k + k] = best.id;
+        taken |= 1u << (best.id / 32);
+        offer();
+      }
+      __syncwarp();
+    }
+  }
+  if (lane == 0) {
+    a.stats[2 * r] = m;
+    a.stats[2 * r + 1] = s;
+    a.entropy[r] = ls - u / s;
+    a.log_probs[r] = target_log_prob(a, r, row, m, ls);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+scores_bwd_warp_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targets,
+                       const T* __restrict__ stats, const T* __restrict__ entropy,
+                       const int64_t* __restrict__ ids, const T* __restrict__ g_log,
+                       const T* __restrict__ g_ent, const T* __restrict__ g_top,
+                       T* __restrict__ grad, int64_t rows, int classes, int top_k,
+                       int64_t ignore_index) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  const Pull<T> p(r, classes, targets, stats, entropy, g_log, g_ent, g_top, top_k, ignore_index);
+  const T* x = logits + r * classes;
+  T* d = grad + r * classes;
+#pragma unroll 8
+  for (int c = lane; c < classes; c += 32) {
+    const T g = p.spread(x[c]);
+    d[c] = c == p.target ? g + p.log : g;
+  }
+  __syncwarp();
+  for (int k = lane; k < top_k; k += 32) d[ids[r * top_k + k]] += g_top[r * top_k + k];
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -449,6 +563,13 @@ int tg_token_log_probs_forward(int dtype, const void* logits, const int64_t* tar
     ScoreArgs<T> a{(const T*)logits, targets, (T*)stats, (T*)log_probs, (T*)entropy,
                    (T*)top_log_probs, top_ids, (int)classes, (int)top_k, 1, (int)classes,
                    ignore_index, bad_target_dev};
+    if (classes <= kWarpRow) {
+      const dim3 grid((unsigned)((rows + kThreads / 32 - 1) / (kThreads / 32)));
+      TG_CUDA_TRY(launch_pdl(classes <= 128 ? scores_fwd_warp_kernel<T, 4>
+                                            : scores_fwd_warp_kernel<T, kWarpRow / 32>,
+                             grid, dim3(kThreads), 0, s, a, rows));
+      return check_launch("token_log_probs");
+    }
     a.splits = row_splits(rows, classes);
     if (a.splits > 1) a.part = (int)((classes + a.splits * VE - 1) / (a.splits * VE) * VE);
     cudaLaunchConfig_t cfg = {};
@@ -481,6 +602,14 @@ int tg_token_log_probs_backward(int dtype, const void* logits, const int64_t* ta
   return TG_DISPATCH_FLOAT(dtype, T, [&] {
     constexpr int VE = 16 / sizeof(T);
     if (!g_top) top_k = 0;  // no gradient comes in through the alternatives
+    if (classes <= kWarpRow) {
+      const dim3 grid((unsigned)((rows + kThreads / 32 - 1) / (kThreads / 32)));
+      TG_CUDA_TRY(launch_pdl(scores_bwd_warp_kernel<T>, grid, dim3(kThreads), 0, s,
+                             (const T*)logits, targets, (const T*)stats, (const T*)entropy,
+                             top_ids, (const T*)g_log, (const T*)g_ent, (const T*)g_top, (T*)grad,
+                             rows, (int)classes, (int)top_k, ignore_index));
+      return check_launch("token_log_probs backward");
+    }
     const int parts = row_splits(rows, classes);
     const int part = (int)((classes + parts * VE - 1) / (parts * VE) * VE);
     const dim3 grid((unsigned)rows, (unsigned)parts);

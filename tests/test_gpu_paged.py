@@ -240,6 +240,32 @@ def test_copy_pages(shape, dtype):
         np.testing.assert_array_equal(pool.numpy(), ref)
 
 
+def test_pools_beyond_32_bit_offsets():
+    import tensorgrad_b200 as tg
+    from tensorgrad_b200 import device
+
+    num = 2**32 // (16 * 64) + 8  # more than 2^32 elements in a pool
+    rng = np.random.default_rng(3)
+    pools = [tg.Tensor._wrap(device.empty((num, 1, 16, 64), np.float32)) for _ in range(2)]
+    table = np.array([[num - 1, num - 4], [5, num - 2]])
+    k, v = rng.standard_normal((2, 2, 1, 20, 64)).astype(np.float32)
+    tg.append_pages(tg.Tensor(k), tg.Tensor(v), *pools, table, [0, 0])
+    held = np.array([20, 20])
+    for got, ref in zip(tg.gather_pages(*pools, table, held, 20), (k, v), strict=True):
+        np.testing.assert_array_equal(got.numpy(), ref)
+    q = rng.standard_normal((2, 3, 64)).astype(np.float32)
+    first = tg.paged_attention(tg.Tensor(q), *pools, table, held).numpy()
+    small = [np.stack([x[b, 0].reshape(-1) for b in range(2)]).reshape(2, 1, 20, 64)
+             for x in (k, v)]
+    ref = tg.paged_attention(tg.Tensor(q), tg.Tensor(small[0]), tg.Tensor(small[1]),
+                             np.array([[0], [1]]), held).numpy()
+    np.testing.assert_array_equal(first, ref)  # which lane has a position is the same
+    tg.copy_pages(*pools, [num - 1, num - 4, 5], [7, num - 5, num - 6])
+    moved = np.array([[7, num - 5], [num - 6, num - 2]])
+    np.testing.assert_array_equal(tg.paged_attention(tg.Tensor(q), *pools, moved, held).numpy(),
+                                  first)
+
+
 # ---------------------------------------------------------------------- the model's path
 def _model(dtype, block=48):
     import tensorgrad_b200 as tg

@@ -63,7 +63,8 @@ def _bounds(x, dtype):
 
 
 SHAPES = [(1, 1, 1), (1, 17, 5), (3, 65, 65), (5, 1000, 20), (2, 4099, 128), (9, 50304, 5),
-          (300, 257, 3), (1, 131072, 20), (700, 1024, 0), (4, 300, 128)]
+          (300, 257, 3), (1, 131072, 20), (700, 1024, 0), (4, 300, 128), (77, 1025, 9),
+          (9, 129, 128), (2, 128, 128)]
 
 
 @pytest.mark.parametrize("dtype", [np.float32, np.float64], ids=["fp32", "fp64"])
@@ -93,7 +94,8 @@ def test_scores_match_definition(rows, classes, top_k, dtype):
 
 @pytest.mark.parametrize("dtype", [np.float32, np.float64], ids=["fp32", "fp64"])
 @pytest.mark.parametrize("rows,classes,top_k", [(1, 1, 1), (3, 65, 7), (5, 4099, 20),
-                                                (300, 257, 0), (2, 50304, 128)])
+                                                (300, 257, 0), (2, 50304, 128), (19, 1025, 3),
+                                                (500, 1024, 2)])
 def test_gradient_matches_formula(rows, classes, top_k, dtype):
     import tensorgrad_b200 as tg
 
@@ -135,7 +137,8 @@ def test_ties_go_to_the_lowest_class():
     import tensorgrad_b200 as tg
 
     rng = np.random.default_rng(0)
-    for rows, classes, top_k in [(3, 5000, 128), (2, 70001, 64), (200, 300, 100), (1, 131, 128)]:
+    for rows, classes, top_k in [(3, 5000, 128), (2, 70001, 64), (200, 300, 100), (1, 131, 128),
+                                 (400, 20000, 30), (5, 1100, 20)]:
         for levels in (1, 3, 40):
             x = rng.integers(0, levels, (rows, classes)).astype(np.float32)
             x[rng.random(x.shape) < 0.1] *= -0.0  # both zeros count as equal
