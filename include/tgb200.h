@@ -442,6 +442,12 @@ int tg_paged_gather(int dtype, int64_t batch, int64_t longest, int64_t kv_heads,
 int tg_page_copy(int64_t page_bytes, int64_t layers, int64_t num_pages, void* key_pages,
                  void* value_pages, const int64_t* src, const int64_t* dst, int64_t pairs,
                  int* bad_page_dev, void* stream);
+/* The same for up to tg_page_copy_few_max() pairs given on the host, which travel with the
+ * launch; an id outside [0, num_pages) is refused (TG_ERR_INDEX) before it. */
+int tg_page_copy_few_max(void);
+int tg_page_copy_few(int64_t page_bytes, int64_t layers, int64_t num_pages, void* key_pages,
+                     void* value_pages, const int64_t* src_host, const int64_t* dst_host,
+                     int64_t pairs, void* stream);
 /* One new token's attention: out (batch, heads, head_dim), contiguous, = softmax(q k^T /
  * sqrt(head_dim)) v over the sequence's first lengths[b] positions, query head h on key head
  * h / (heads / kv_heads); lse (batch, heads; may be NULL) = the log-sum-exp of the scaled

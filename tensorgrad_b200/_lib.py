@@ -166,6 +166,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                 vp, vp, i64, i64, vp, i64, vp, vp, vp]),
     "tg_paged_gather": (c_int, [c_int, i64, i64, i64, i64, vp, vp, i64, i64, vp, i64, vp, vp, vp,
                                 vp, vp]),
+    "tg_page_copy_few_max": (c_int, []),
+    "tg_page_copy_few": (c_int, [i64, i64, i64, vp, vp, vp, vp, i64, vp]),
     "tg_page_copy": (c_int, [i64, i64, i64, vp, vp, vp, vp, i64, vp, vp]),
     "tg_paged_attention_scratch_bytes": (sz, [c_int, i64, i64, i64, i64, i64]),
     "tg_paged_attention": (c_int, [c_int, i64, i64, i64, i64, vp, i64, i64, vp, vp, i64, i64, vp,

@@ -127,22 +127,36 @@ gather_kernel(Moves m, const V* __restrict__ keys, const V* __restrict__ values,
 // Pages src[i] to dst[i] in every layer of both pools; `units` of V to a page. Pages of 256 units
 // and more take a block or several (1024 pages of 48 KB in 12 layers: 6.1 TB/s), shorter ones share
 // one.
-template <typename V>
+// Up to kInline pairs travel with the launch, more of them lie on the device.
+constexpr int kInline = 64;
+
+struct Pairs {
+  const int64_t* src;
+  const int64_t* dst;
+  __device__ __forceinline__ int64_t from(int64_t i) const { return src[i]; }
+  __device__ __forceinline__ int64_t to(int64_t i) const { return dst[i]; }
+};
+struct InlinePairs {
+  int src[kInline], dst[kInline];
+  __device__ __forceinline__ int64_t from(int64_t i) const { return src[i]; }
+  __device__ __forceinline__ int64_t to(int64_t i) const { return dst[i]; }
+};
+
+template <typename V, typename P>
 struct Copies {
   V* keys;
   V* values;
   int64_t layers, num_pages, units;
-  const int64_t* src;
-  const int64_t* dst;
+  P ids;
   int64_t pairs;
   int* bad;
 };
 
 // Where copy e of 2 layers pairs reads and writes; false behind a bad id.
-template <typename V>
-__device__ __forceinline__ bool place_of(const Copies<V>& c, int64_t l, int64_t i, const V*& from,
-                                         V*& to) {
-  const int64_t a = c.src[i], b = c.dst[i];
+template <typename V, typename P>
+__device__ __forceinline__ bool place_of(const Copies<V, P>& c, int64_t l, int64_t i,
+                                         const V*& from, V*& to) {
+  const int64_t a = c.ids.from(i), b = c.ids.to(i);
   if (a < 0 || a >= c.num_pages || b < 0 || b >= c.num_pages) {
     if (c.bad) *c.bad = 1;
     return false;
@@ -154,9 +168,9 @@ __device__ __forceinline__ bool place_of(const Copies<V>& c, int64_t l, int64_t 
   return true;
 }
 
-template <typename V>
+template <typename V, typename P>
 __global__ void __launch_bounds__(kThreads)
-page_copy_kernel(Copies<V> c, int parts, int64_t part) {
+page_copy_kernel(const __grid_constant__ Copies<V, P> c, int parts, int64_t part) {
   const int64_t total = 2 * c.layers * c.pairs * parts;
   for (int64_t e = blockIdx.x; e < total; e += gridDim.x) {
     const int64_t p = e / parts, first = e % parts * part;
@@ -169,9 +183,9 @@ page_copy_kernel(Copies<V> c, int parts, int64_t part) {
   }
 }
 
-template <typename V>
+template <typename V, typename P>
 __global__ void __launch_bounds__(kThreads)
-page_copy_short_kernel(Copies<V> c, int total, FastDiv units, FastDiv pairs) {
+page_copy_short_kernel(const __grid_constant__ Copies<V, P> c, int total, FastDiv units, FastDiv pairs) {
   for (int e = blockIdx.x * kThreads + threadIdx.x; e < total; e += (int)gridDim.x * kThreads) {
     const int p = div_by(e, units), l = div_by(p, pairs);
     const V* from;
@@ -763,20 +777,30 @@ int launch_gather(const Moves& m, const V* keys, const V* values, V* k, V* v, cu
   });
 }
 
-template <typename V>
-int launch_copies(const Copies<V>& c, cudaStream_t s) {
+template <typename V, typename P>
+int launch_copies(const Copies<V, P>& c, cudaStream_t s) {
   const int64_t pages = 2 * c.layers * c.pairs;
   if (c.units < kThreads && pages * c.units <= INT32_MAX / 2)
-    page_copy_short_kernel<V><<<grid_for(pages * c.units, kThreads), kThreads, 0, s>>>(
+    page_copy_short_kernel<<<grid_for(pages * c.units, kThreads), kThreads, 0, s>>>(
         c, (int)(pages * c.units), make_div(c.units), make_div(c.pairs));
   else {
     // Few pages are cut into parts of at least 4 units a lane.
     const int64_t most = (c.units + 4 * kThreads - 1) / (4 * kThreads);
     const int64_t want = (148 * 8 + pages - 1) / pages;
     const int64_t parts = want < most ? want : most, part = (c.units + parts - 1) / parts;
-    page_copy_kernel<V><<<grid_for(pages * parts, 1), kThreads, 0, s>>>(c, (int)parts, part);
+    page_copy_kernel<<<grid_for(pages * parts, 1), kThreads, 0, s>>>(c, (int)parts, part);
   }
   return check_launch("page_copy");
+}
+
+template <typename P>
+int copy_pages(int64_t page_bytes, int64_t layers, int64_t num_pages, void* key_pages,
+               void* value_pages, const P& ids, int64_t pairs, int* bad, cudaStream_t s) {
+  if (page_bytes % 16 == 0 && aligned16(key_pages) && aligned16(value_pages))
+    return launch_copies(Copies<Unit16, P>{(Unit16*)key_pages, (Unit16*)value_pages, layers,
+                                           num_pages, page_bytes / 16, ids, pairs, bad}, s);
+  return launch_copies(Copies<uint32_t, P>{(uint32_t*)key_pages, (uint32_t*)value_pages, layers,
+                                           num_pages, page_bytes / 4, ids, pairs, bad}, s);
 }
 
 }  // namespace
@@ -846,14 +870,30 @@ int tg_page_copy(int64_t page_bytes, int64_t layers, int64_t num_pages, void* ke
   TG_CHECK_ARG(page_bytes > 0 && page_bytes % 4 == 0 && layers > 0 && num_pages > 0 && pairs >= 0,
                "page_copy: bad sizes");
   if (pairs == 0) return TG_OK;
-  cudaStream_t s = as_stream(stream);
-  if (page_bytes % 16 == 0 && aligned16(key_pages) && aligned16(value_pages))
-    return launch_copies(Copies<Unit16>{(Unit16*)key_pages, (Unit16*)value_pages, layers,
-                                        num_pages, page_bytes / 16, src, dst, pairs,
-                                        bad_page_dev}, s);
-  return launch_copies(Copies<uint32_t>{(uint32_t*)key_pages, (uint32_t*)value_pages, layers,
-                                        num_pages, page_bytes / 4, src, dst, pairs,
-                                        bad_page_dev}, s);
+  return copy_pages(page_bytes, layers, num_pages, key_pages, value_pages, Pairs{src, dst}, pairs,
+                    bad_page_dev, as_stream(stream));
+}
+
+int tg_page_copy_few_max(void) { return kInline; }
+
+int tg_page_copy_few(int64_t page_bytes, int64_t layers, int64_t num_pages, void* key_pages,
+                     void* value_pages, const int64_t* src_host, const int64_t* dst_host,
+                     int64_t pairs, void* stream) {
+  TG_CHECK_ARG(page_bytes > 0 && page_bytes % 4 == 0 && layers > 0 && num_pages > 0 &&
+                   num_pages <= INT32_MAX && pairs >= 0 && pairs <= kInline,
+               "page_copy_few: bad sizes");
+  if (pairs == 0) return TG_OK;
+  InlinePairs ids;
+  for (int64_t i = 0; i < pairs; ++i) {
+    if (src_host[i] < 0 || src_host[i] >= num_pages || dst_host[i] < 0 ||
+        dst_host[i] >= num_pages)
+      return set_error(TG_ERR_INDEX, "page_copy_few: pages %lld and %lld of %lld",
+                       (long long)src_host[i], (long long)dst_host[i], (long long)num_pages);
+    ids.src[i] = (int)src_host[i];
+    ids.dst[i] = (int)dst_host[i];
+  }
+  return copy_pages(page_bytes, layers, num_pages, key_pages, value_pages, ids, pairs, nullptr,
+                    as_stream(stream));
 }
 
 size_t tg_paged_attention_scratch_bytes(int dtype, int64_t batch, int64_t heads, int64_t kv_heads,

@@ -27,6 +27,8 @@ from tensorgrad_b200.tensor import Tensor
 
 __all__ = ["append_pages", "copy_pages", "gather_pages", "paged_attention"]
 
+_FEW_PAIRS = 64  # at most tg_page_copy_few_max(): their ids travel with the launch
+
 
 def _inference_only(what: str, *tensors: Tensor) -> None:
     if is_grad_enabled() and any(t.requires_grad for t in tensors):
@@ -152,27 +154,41 @@ def copy_pages(keys: Tensor, values: Tensor, src: Any, dst: Any) -> None:
     destination is written once and is not a source of the same call."""
     pk, pv = _pools("copy_pages", keys, values, (4, 5))
     _inference_only("copy_pages", pk, pv)
-    a, b = np.atleast_1d(np.asarray(src)), np.atleast_1d(np.asarray(dst))
-    if a.size == 0 and b.size == 0:
+    a, b = np.asarray(src), np.asarray(dst)
+    if a.ndim != 1 or a.shape != b.shape:
+        raise ValueError(f"copy_pages: expected lists of as many sources as destinations, got "
+                         f"{a.shape} and {b.shape}")
+    n = a.size
+    if n == 0:
         return
     if a.dtype.kind not in "iu" or b.dtype.kind not in "iu":
         raise TypeError(f"copy_pages: page ids must be integers, got {a.dtype} and {b.dtype}")
-    if a.ndim != 1 or a.shape != b.shape:
-        raise ValueError(f"copy_pages: sources {a.shape} and destinations {b.shape} differ")
     layers = pk.shape[0] if pk.ndim == 5 else 1
     num_pages, heads, size, width = pk.shape[-4:]
-    if min(a.min(), b.min()) < 0 or max(a.max(), b.max()) >= num_pages:
+    pairs = np.empty((2, n), dtype=np.int64)
+    pairs[0], pairs[1] = a, b
+    if pairs.min() < 0 or pairs.max() >= num_pages:
         raise IndexError(f"copy_pages: page ids must be in [0, {num_pages})")
-    written = np.zeros(num_pages, dtype=np.bool_)
-    written[b] = True
-    if np.count_nonzero(written) != b.size:
+    few = n <= _FEW_PAIRS
+    if few:
+        to = set(pairs[1].tolist())
+        distinct, apart = len(to) == n, to.isdisjoint(pairs[0].tolist())
+    else:
+        written = np.zeros(num_pages, dtype=np.bool_)
+        written[pairs[1]] = True
+        distinct, apart = np.count_nonzero(written) == n, not written[pairs[0]].any()
+    if not distinct:
         raise ValueError("copy_pages: a destination page is given twice")
-    if written[a].any():
+    if not apart:
         raise ValueError("copy_pages: a page is both a source and a destination")
-    ids = device.from_numpy(np.stack([a, b]).astype(np.int64))
-    check(lib.tg_page_copy(heads * size * width * pk.dtype.itemsize, layers, num_pages,
-                           pk.data.ptr, pv.data.ptr, ids.ptr, ids.ptr + 8 * a.size, a.size, None,
-                           device.stream()), "copy_pages")
+    where = (heads * size * width * pk.dtype.itemsize, layers, num_pages, pk.data.ptr, pv.data.ptr)
+    if few:
+        at = pairs.ctypes.data
+        check(lib.tg_page_copy_few(*where, at, at + 8 * n, n, device.stream()), "copy_pages")
+        return
+    ids = device.from_numpy(pairs)
+    check(lib.tg_page_copy(*where, ids.ptr, ids.ptr + 8 * n, n, None, device.stream()),
+          "copy_pages")
 
 
 def attend_strided(batch: int, heads: int, q: tuple[int, tuple[int, int]], keys: DeviceArray,

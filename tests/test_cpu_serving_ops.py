@@ -114,8 +114,9 @@ def test_page_ops_refuse_bad_arguments():
         copy_pages(pool, pool, [0, 1], [2, 2])
     with pytest.raises(ValueError, match="both a source"):
         copy_pages(pool, pool, [0, 1], [1, 2])
-    with pytest.raises(ValueError, match="differ"):
-        copy_pages(pool, pool, [0, 1], [2])
+    for src, dst in (([0, 1], [2]), (0, 1), ([[0]], [[1]])):
+        with pytest.raises(ValueError, match="as many sources"):
+            copy_pages(pool, pool, src, dst)
     with pytest.raises(TypeError, match="integers"):
         copy_pages(pool, pool, [0.5], [2.0])
     copy_pages(pool, pool, [], [])
@@ -141,6 +142,17 @@ def test_page_entry_points_refuse_bad_sizes():
     assert attend(width=257) == 3
     assert lib.tg_page_copy(6, 1, 4, None, None, None, None, 1, None, None) == 1
     assert lib.tg_page_copy(8, 1, 4, None, None, None, None, 0, None, None) == 0
+    import ctypes
+
+    from tensorgrad_b200.ops.paged import _FEW_PAIRS
+
+    assert 0 < _FEW_PAIRS <= lib.tg_page_copy_few_max()
+    ids = (ctypes.c_int64 * 2)(0, 4)
+    at = ctypes.addressof(ids)
+    assert lib.tg_page_copy_few(8, 1, 4, None, None, at, at + 8, 1, None) == 4
+    assert lib.tg_page_copy_few(8, 1, 4, None, None, at + 8, at, 1, None) == 4
+    assert lib.tg_page_copy_few(8, 1, 4, None, None, None, None, 65, None) == 1
+    assert lib.tg_page_copy_few(8, 1, 4, None, None, None, None, 0, None) == 0
     assert lib.tg_paged_gather(0, 1, -1, 1, 1, None, None, 1, 1, None, 1, None, None, None, None,
                                None) == 1
 

@@ -223,7 +223,9 @@ def test_append_then_gather(tokens, kv_heads, width, size, dtype):
     np.testing.assert_array_equal(short, got[0].numpy()[:, :, :2])
 
 
-@pytest.mark.parametrize("shape", [(6, 2, 4, 8), (3, 7, 1, 5, 3), (12, 40, 4, 16, 64)])
+@pytest.mark.parametrize("shape", [(6, 2, 4, 8), (3, 7, 1, 5, 3), (12, 40, 4, 16, 64),
+                                   (128, 1, 16, 64), (2, 130, 1, 7, 33), (3, 400, 2, 16, 80),
+                                   (5000, 1, 1, 1)])
 def test_copy_pages(shape, dtype):
     import tensorgrad_b200 as tg
 
