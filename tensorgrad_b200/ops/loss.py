@@ -212,8 +212,9 @@ def _class_targets(what: str, tl: Tensor, target: Any,
     if tl.shape[:-1] != t.shape:
         raise ValueError(f"logits {tl.shape} and targets {t.shape} are incompatible")
     if on_device:
-        tgt = t if t.dtype == np.int64 else cast_array(t, np.dtype(np.int64))
-        return tgt, device.async_error_word(device.ASYNC_CLASS_TARGET)
+        if t.dtype != np.int64:
+            raise TypeError(f"{what} targets on the device must be int64, got {t.dtype}")
+        return t, device.async_error_word(device.ASYNC_CLASS_TARGET)
     flat = np.ascontiguousarray(t.reshape(-1), dtype=np.int64)
     if np.any((flat != ignore_index) & ((flat < 0) | (flat >= tl.shape[-1]))):
         raise IndexError(f"target out of range for {tl.shape[-1]} classes")

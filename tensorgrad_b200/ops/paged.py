@@ -60,6 +60,8 @@ def _table(what: str, pages: Any, lengths: Any, batch: int, num_pages: int, page
     for name, x in (("pages", table), ("lengths", held)):
         if x.dtype.kind not in "iu":
             raise TypeError(f"{what}: {name} must be integers, got {x.dtype}")
+        if isinstance(x, DeviceArray) and x.dtype != np.int64:
+            raise TypeError(f"{what}: {name} on the device must be int64, got {x.dtype}")
     if len(table.shape) != 2 or table.shape[0] != batch or table.shape[1] == 0:
         raise ValueError(f"{what}: expected pages ({batch}, max_pages), got {table.shape}")
     if tuple(held.shape) != (batch,):
@@ -75,12 +77,8 @@ def _table(what: str, pages: Any, lengths: Any, batch: int, num_pages: int, page
             if ids.size and (ids.min() < 0 or ids.max() >= num_pages):
                 raise IndexError(f"{what}: page ids must be in [0, {num_pages})")
     checked = isinstance(table, np.ndarray) and isinstance(held, np.ndarray)
-    out = []
-    for x in (table, held):
-        if isinstance(x, np.ndarray):
-            out.append(device.from_numpy(np.ascontiguousarray(x, dtype=np.int64)))
-        else:
-            out.append(x if x.dtype == np.int64 else x.astype(np.int64))
+    out = [device.from_numpy(np.ascontiguousarray(x, dtype=np.int64))
+           if isinstance(x, np.ndarray) else x for x in (table, held)]
     bad = None if checked else device.async_error_word(device.ASYNC_CACHE_PAGE)
     return out[0], out[1], bad
 
