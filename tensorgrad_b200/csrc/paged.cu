@@ -223,6 +223,83 @@ struct Base<double> {
   static __device__ __forceinline__ double natural(double x) { return x; }
 };
 
+// A lane's 8 features. Floats are kept and multiplied two to an instruction (fma.rn.f32x2: half the
+// issue slots, the same roundings).
+template <typename T>
+struct Eight {
+  T v[kLaneDims];
+  __device__ __forceinline__ void set(const T (&x)[kLaneDims]) {
+#pragma unroll
+    for (int i = 0; i < kLaneDims; ++i) v[i] = x[i];
+  }
+  __device__ __forceinline__ T get(int i) const { return v[i]; }
+  __device__ __forceinline__ T dot(const Eight& o) const {
+    T s = v[0] * o.v[0];
+#pragma unroll
+    for (int i = 1; i < kLaneDims; ++i) s += v[i] * o.v[i];
+    return s;
+  }
+  __device__ __forceinline__ void add(T f, const Eight& o) {
+#pragma unroll
+    for (int i = 0; i < kLaneDims; ++i) v[i] += f * o.v[i];
+  }
+  __device__ __forceinline__ void scale(T f) {
+#pragma unroll
+    for (int i = 0; i < kLaneDims; ++i) v[i] *= f;
+  }
+};
+
+template <>
+struct Eight<float> {
+  using Two = unsigned long long;
+  Two p[kLaneDims / 2];
+  static __device__ __forceinline__ Two pack(float a, float b) {
+    Two r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+  }
+  static __device__ __forceinline__ float2 unpack(Two x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+  }
+  static __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+  }
+  static __device__ __forceinline__ Two mul2(Two a, Two b) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+  }
+  __device__ __forceinline__ void set(const float (&x)[kLaneDims]) {
+#pragma unroll
+    for (int i = 0; i < kLaneDims / 2; ++i) p[i] = pack(x[2 * i], x[2 * i + 1]);
+  }
+  __device__ __forceinline__ float get(int i) const {
+    const float2 x = unpack(p[i / 2]);
+    return i % 2 ? x.y : x.x;
+  }
+  __device__ __forceinline__ float dot(const Eight& o) const {
+    Two s = mul2(p[0], o.p[0]);
+#pragma unroll
+    for (int i = 1; i < kLaneDims / 2; ++i) s = fma2(p[i], o.p[i], s);
+    const float2 x = unpack(s);
+    return x.x + x.y;
+  }
+  __device__ __forceinline__ void add(float f, const Eight& o) {
+    const Two both = pack(f, f);
+#pragma unroll
+    for (int i = 0; i < kLaneDims / 2; ++i) p[i] = fma2(both, o.p[i], p[i]);
+  }
+  __device__ __forceinline__ void scale(float f) {
+    const Two both = pack(f, f);
+#pragma unroll
+    for (int i = 0; i < kLaneDims / 2; ++i) p[i] = mul2(p[i], both);
+  }
+};
+
 template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t to, const void* from, bool live) {
   const int n = live ? BYTES : 0;  // nothing read, zeros written
@@ -293,7 +370,7 @@ struct Attend {
 };
 
 template <typename T, int VE, int LPT, int GH>
-__global__ void __launch_bounds__(kAttend, GH == 8 ? 2 : 4)
+__global__ void __launch_bounds__(kAttend, 4)
 paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restrict__ keys,
                        const T* __restrict__ values, T* __restrict__ out, T* __restrict__ lse,
                        T* __restrict__ part) {
@@ -301,6 +378,9 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
   constexpr int NVEC = A::NVEC, ST = A::ST, TPW = 32 / LPT, ROWS = kWarps * TPW, STEP = U * ROWS;
   constexpr int V = A::V, KEPT = A::KEPT;
   constexpr T kLowest = std::numeric_limits<T>::lowest();
+  struct alignas(A::VB) Held {
+    T v[VE];
+  };
   extern __shared__ __align__(16) uint8_t smem[];
   int64_t* table = reinterpret_cast<int64_t*>(smem + A::SMEM - kTable * 8);
   pdl_trigger();
@@ -324,17 +404,21 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
   // m and l belong to the KEPT scores that this lane finishes: the running maximum of that
   // score's head (the same in every lane of the group that has the head) and the sum over the
   // positions that came to this lane.
-  T qr[GH][kLaneDims], acc[GH][kLaneDims], m[KEPT], l[KEPT];
+  Eight<T> qr[GH], acc[GH];
+  T m[KEPT], l[KEPT];
 #pragma unroll
-  for (int g = 0; g < GH; ++g)
+  for (int g = 0; g < GH; ++g) {
+    T x[kLaneDims], zero[kLaneDims] = {};
 #pragma unroll
     for (int i = 0; i < kLaneDims; ++i) {
       const int c = ((i / VE) * LPT + j) * VE + i % VE;
-      qr[g][i] = g < live_heads && c < d
-                     ? q[b * a.q_sb + (h0 + g) * a.q_sh + c] * (T)(a.scale * Base<T>::unit)
-                     : T(0);
-      acc[g][i] = T(0);
+      x[i] = g < live_heads && c < d
+                 ? q[b * a.q_sb + (h0 + g) * a.q_sh + c] * (T)(a.scale * Base<T>::unit)
+                 : T(0);
     }
+    qr[g].set(x);
+    acc[g].set(zero);
+  }
 #pragma unroll
   for (int r = 0; r < KEPT; ++r) {
     m[r] = kLowest;
@@ -396,25 +480,24 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
     for (int i = 0; i < steps; ++i) {
       copy_wait<ST - 2>();
       const uint8_t* from = mine + (i % ST) * A::STAGE;
-      auto load = [&](T (&x)[kLaneDims], const uint8_t* row) {
+      auto load = [&](const uint8_t* row) {
+        T x[kLaneDims];
 #pragma unroll
-        for (int v = 0; v < NVEC; ++v)
+        for (int v = 0; v < NVEC; ++v) {
+          const Held y = *reinterpret_cast<const Held*>(row + v * (A::VB * kAttend));
 #pragma unroll
-          for (int c = 0; c < VE; ++c)
-            x[v * VE + c] = reinterpret_cast<const T*>(row + v * (A::VB * kAttend))[c];
+          for (int c = 0; c < VE; ++c) x[v * VE + c] = y.v[c];
+        }
+        Eight<T> e;
+        e.set(x);
+        return e;
       };
       T s[V];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        T x[kLaneDims];
-        load(x, from + u * A::ROW);
+        const Eight<T> x = load(from + u * A::ROW);
 #pragma unroll
-        for (int g = 0; g < GH; ++g) {
-          T dot = T(0);
-#pragma unroll
-          for (int c = 0; c < kLaneDims; ++c) dot += qr[g][c] * x[c];
-          s[u * GH + g] = dot;
-        }
+        for (int g = 0; g < GH; ++g) s[u * GH + g] = qr[g].dot(x);
       }
 #pragma unroll
       for (int k = 0; k < log2_of(LPT); ++k) {
@@ -454,9 +537,7 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
         }
 #pragma unroll
         for (int g = 0; g < GH; ++g) {
-          const T cg = __shfl_sync(0xffffffffu, c[g % KEPT], sub * LPT + A::lane_of(g));
-#pragma unroll
-          for (int k = 0; k < kLaneDims; ++k) acc[g][k] *= cg;
+          acc[g].scale(__shfl_sync(0xffffffffu, c[g % KEPT], sub * LPT + A::lane_of(g)));
         }
       }
 #pragma unroll
@@ -466,14 +547,11 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        T x[kLaneDims];
-        load(x, from + u * A::ROW + NVEC * (A::VB * kAttend));
+        const Eight<T> x = load(from + u * A::ROW + NVEC * (A::VB * kAttend));
 #pragma unroll
         for (int g = 0; g < GH; ++g) {
           const int v = u * GH + g;
-          const T p = __shfl_sync(0xffffffffu, s[v % KEPT], sub * LPT + A::lane_of(v));
-#pragma unroll
-          for (int k = 0; k < kLaneDims; ++k) acc[g][k] += p * x[k];
+          acc[g].add(__shfl_sync(0xffffffffu, s[v % KEPT], sub * LPT + A::lane_of(v)), x);
         }
       }
       if (i + ST - 1 < steps) issue(i + ST - 1);
@@ -485,9 +563,11 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
 
   // Every lane learns its heads' maxima and sums, then the warp's lane groups join, then the
   // block's warps.
-  T mg[GH], lg[GH];
+  T mg[GH], lg[GH], og[GH][kLaneDims];
 #pragma unroll
   for (int g = 0; g < GH; ++g) {
+#pragma unroll
+    for (int k = 0; k < kLaneDims; ++k) og[g][k] = acc[g].get(k);
     mg[g] = __shfl_sync(0xffffffffu, m[g % KEPT], sub * LPT + A::lane_of(g));
     lg[g] = T(0);
 #pragma unroll
@@ -505,8 +585,8 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
       mg[g] = top;
 #pragma unroll
       for (int k = 0; k < kLaneDims; ++k) {
-        acc[g][k] *= c;
-        acc[g][k] += __shfl_xor_sync(0xffffffffu, acc[g][k], o);
+        og[g][k] *= c;
+        og[g][k] += __shfl_xor_sync(0xffffffffu, og[g][k], o);
       }
     }
   __syncthreads();
@@ -518,7 +598,7 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
     for (int g = 0; g < GH; ++g) {
 #pragma unroll
       for (int k = 0; k < kLaneDims; ++k)
-        sacc[(w * GH + g) * A::WIDTH + ((k / VE) * LPT + j) * VE + k % VE] = acc[g][k];
+        sacc[(w * GH + g) * A::WIDTH + ((k / VE) * LPT + j) * VE + k % VE] = og[g][k];
       if (j == 0) {
         sm[w * GH + g] = mg[g];
         sl[w * GH + g] = lg[g];
@@ -639,9 +719,11 @@ int sm_count() {
 }
 
 // Query heads that one block takes: the group of a key head, rounded up to a power of two, at
-// most 8 (2 where the lanes hold double: more would not fit the registers).
+// most 4 (2 where the lanes hold double): 8 leave half as many warps for the registers, and two
+// blocks that share keys and values through the L2 are faster (8 heads of 64 to a key head, 64 x 4
+// of them up to 4096 positions: 190 us with 8, 116 with 4 a block).
 int heads_per_block(int dtype, int64_t group) {
-  const int most = dtype == TG_F64 ? 2 : 8;
+  const int most = dtype == TG_F64 ? 2 : 4;
   int g = 1;
   while (g < group && g < most) g *= 2;
   return g;
@@ -696,11 +778,8 @@ int attend_heads(int gh, const AttendArgs& a, int64_t blocks, const T* q, const 
     case 1: return launch_attend<T, VE, LPT, 1>(a, blocks, q, keys, values, out, lse, part, s);
     case 2: return launch_attend<T, VE, LPT, 2>(a, blocks, q, keys, values, out, lse, part, s);
   }
-  if constexpr (sizeof(T) == 4) {
-    if (gh == 4)
-      return launch_attend<T, VE, LPT, 4>(a, blocks, q, keys, values, out, lse, part, s);
-    return launch_attend<T, VE, LPT, 8>(a, blocks, q, keys, values, out, lse, part, s);
-  }
+  if constexpr (sizeof(T) == 4)
+    return launch_attend<T, VE, LPT, 4>(a, blocks, q, keys, values, out, lse, part, s);
   return set_error(TG_ERR_UNSUPPORTED, "paged_attention: %d heads to a block", gh);
 }
 
