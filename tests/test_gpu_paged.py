@@ -83,6 +83,9 @@ CASES = [
     ([50, 2], 7, 1, 1, 3),
     ([777], 24, 2, 255, 9),
     ([4000, 4096, 12], 4, 2, 8, 16),
+    ([900, 33, 0, 5000], 10, 2, 128, 16),
+    ([200] * 9, 64, 8, 64, 8),
+    ([3000, 2], 24, 3, 33, 16),
 ]
 
 
