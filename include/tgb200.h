@@ -397,10 +397,11 @@ int tg_attention_backward_dropout(int dtype, const tg_attn_shape* s, const void*
 
 /* ------------------------------------------------------------------ 8-bit integer linear
  * The inference form of ops/layers.py:22-62 with a scale for each token and each channel (no
- * reference counterpart). tg_int8_quantize_rows: scales[r] = max|x[r]| / 127, q[r][c] = the
- * nearest integer to x[r][c] / scales[r] (halves to even, quotient rounded to the type first),
- * rows of ld >= inner bytes with zeros behind the values. A row of zeros has scale 0 and
- * integers 0, a row with a NaN or an infinity scale NaN and integers 0. */
+ * reference counterpart). tg_int8_quantize_rows: scales[r] = max|x[r]| * (1 / 127), the factor
+ * rounded to the type; q[r][c] = the nearest integer to x[r][c] / scales[r] (halves to even,
+ * quotient rounded to the type first), rows of ld >= inner bytes with zeros behind the values. A
+ * row of zeros has scale 0 and integers 0, a row with a NaN or an infinity scale NaN and
+ * integers 0. */
 int tg_int8_quantize_rows(int dtype, const void* x, int64_t rows, int64_t inner, int8_t* q,
                           int64_t ld, void* scales, void* stream);
 /* y (rows, outer) = (q(x) w^T) (scale of the row * scales[channel]) + bias (may be NULL), the

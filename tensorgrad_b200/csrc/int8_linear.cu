@@ -1,6 +1,6 @@
 // Linear layers in 8-bit integers (no reference counterpart; the inference form of
 // ops/layers.py:22-62): a scale for each token and each output channel,
-//   s_m = max_k |x_mk| / 127,  q_mk = rint(x_mk / s_m),
+//   s_m = max_k |x_mk| * (1 / 127),  q_mk = rint(x_mk / s_m),
 //   y_mn = (sum_k q_mk w_nk) (s_m s_n) + bias_n,
 // the sums exact in 32-bit integers (at most 127 * 128 * 131072 < 2^31). A row of zeros has scale
 // 0 and integers 0; a row with a NaN or an infinity has scale NaN, so its outputs are NaN.
@@ -54,10 +54,11 @@ struct Reciprocal {
   }
 };
 
-// A row's scale from its largest magnitude; `odd` is NaN if the row has a NaN or an infinity.
+// A row's scale from its largest magnitude, times 1 / 127 as the type rounds it; `odd` is NaN if
+// the row has a NaN or an infinity.
 template <typename T>
 __device__ __forceinline__ T scale_of(T top, T odd) {
-  return top / T(127) + odd;
+  return top * T(1.0 / 127) + odd;
 }
 
 // Row scales and integers; integer rows are ld bytes long, zero beyond the row's values.

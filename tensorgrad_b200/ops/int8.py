@@ -2,7 +2,7 @@
 ops/layers.py:22-62 that serves a trained model).
 
 The weight is quantised once, each output channel by its own scale; the input is quantised in
-the call, each token (row) by its own: ``scale = max|x| / 127`` and the nearest integers to
+the call, each token (row) by its own: ``scale = max|x| * (1 / 127)`` and the nearest integers to
 ``x / scale``. The products are summed exactly in 32-bit integers and scaled once.
 """
 
@@ -98,9 +98,9 @@ def _quantize_rows(x: DeviceArray, ld: int) -> tuple[DeviceArray, DeviceArray]:
 @profiled("quantize_int8")
 def quantize_int8(x: Any) -> tuple[Tensor, Tensor]:
     """``x`` over its last axis as 8-bit integers of ``x``'s shape and one scale per row
-    (``x.shape[:-1]``): ``scale = max|row| / 127`` and the nearest integers to ``row / scale``,
-    halves to even. A row of zeros has scale 0; a row with a NaN or an infinity has scale NaN
-    and integers 0."""
+    (``x.shape[:-1]``): ``scale = max|row| * (1 / 127)``, the factor rounded to the type, and
+    the nearest integers to ``row / scale`` rounded to the type, halves to even. A row of zeros
+    has scale 0; a row with a NaN or an infinity has scale NaN and integers 0."""
     tx = as_tensor(x)
     if tx.ndim == 0 or tx.shape[-1] == 0:
         raise ValueError(f"quantize_int8 needs a last axis with values, got {tx.shape}")

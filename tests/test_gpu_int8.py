@@ -21,7 +21,7 @@ def dtype(request):
 
 def _quantized(x):
     """(integers, scales) as the type of ``x`` rounds them."""
-    scale = np.abs(x).max(-1) / x.dtype.type(127)
+    scale = np.abs(x).max(-1) * (x.dtype.type(1) / x.dtype.type(127))
     safe = np.where(scale > 0, scale, 1)[..., None].astype(x.dtype)
     q = np.clip(np.rint(x / safe), -127, 127) * (scale > 0)[..., None]
     return q.astype(np.int8), scale
