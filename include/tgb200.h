@@ -323,7 +323,7 @@ int tg_cross_entropy_backward(int dtype, const void* logits, const int64_t* targ
 
 /* ------------------------------------------------------------------ scores of tokens
  * Under logits (rows, classes), class axis last (no reference counterpart): per row, with m =
- * max x and s = sum exp(x - m) written to stats[row] = (m, s) for the VJP,
+ * max x and s = sum exp(x - m) written to stats[row] = (m, s - 1) for the VJP,
  *   log_probs[row] = x[t] - m - log s  (0 where t == ignore_index; a target outside [0, classes)
  *                    that is not ignore_index sets *bad_target_dev, int32, and gives 0),
  *   entropy[row]   = -sum p log p,

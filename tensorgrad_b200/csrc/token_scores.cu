@@ -3,8 +3,10 @@
 //   log p_t  = (x_t - m) - log s                     the given token
 //   H        = log s - (1 / s) sum e^(x - m) (x - m) the entropy of the whole distribution
 //   (log p_i, i) of the k largest x_i, equal ones by ascending i
-// and their VJP. Row statistics m and s are kept apart for the VJP (p = e^(x - m) / s): folding
-// them into one log-sum-exp would round p to that sum's spacing.
+// and their VJP. The largest entry's own 1 is kept out of the sum: r = s - 1 and log1p(r) hold the
+// log probability and the entropy of a nearly certain token to their last digits, where 1 + r
+// would have rounded r away. m and r are kept apart for the VJP (p = e^(x - m) / (1 + r)): one
+// log-sum-exp would round p to that sum's spacing.
 #include <cooperative_groups.h>
 
 #include <limits>
@@ -56,43 +58,53 @@ __device__ __forceinline__ bool before(Alt<U> a, Alt<U> b) {
 }
 
 // ---------------------------------------------------------------- row statistics
-// Running maximum m (the type's lowest value before the first), s = sum e^(x - m) and
-// u = sum e^(x - m) (x - m).
+// Running maximum m (the type's lowest value before the first), r = sum e^(x - m) - 1 without the
+// rounding of that 1 (-1 before the first) and u = sum e^(x - m) (x - m).
 template <typename T>
 struct Stats {
-  T m, s, u;
+  T m, r, u;
 };
 
 template <typename T>
 constexpr T kLowest = std::numeric_limits<T>::lowest();
 
+template <typename T>
+__device__ __forceinline__ Stats<T> no_stats() {
+  return {kLowest<T>, T(-1), T(0)};
+}
+
 // e^x for x <= 0. The float form multiplies by log2 e in the argument: off by (4 + 2.4 |x|) half
 // steps, and a term of size |x| weighs e^x.
 __device__ __forceinline__ float exp_below(float x) { return __expf(x); }
 __device__ __forceinline__ double exp_below(double x) { return exp(x); }
+__device__ __forceinline__ float log_1p(float x) { return log1pf(x); }
+__device__ __forceinline__ double log_1p(double x) { return log1p(x); }
 
-// The statistics of two sets of values as one. Shifting a maximum from m to m' >= m scales every
-// e^(x - m) by c = e^(m - m') and moves every x - m by m - m'.
+// The statistics of two sets of values as one: the lower maximum's set is scaled by
+// c = e^(its m - the other m), every x - m of it moves by the difference.
 template <typename T>
 __device__ __forceinline__ Stats<T> join(Stats<T> a, Stats<T> b) {
-  Stats<T> r{fmax(a.m, b.m), T(0), T(0)};
-  if (a.s != T(0)) {
-    const T d = a.m - r.m, c = exp_below(d);
-    r.s += a.s * c;
-    r.u += c * (a.u + a.s * d);
+  if (b.m > a.m) {
+    const Stats<T> t = a;
+    a = b;
+    b = t;
   }
-  if (b.s != T(0)) {
-    const T d = b.m - r.m, c = exp_below(d);
-    r.s += b.s * c;
-    r.u += c * (b.u + b.s * d);
-  }
-  return r;
+  const T s = T(1) + b.r;
+  if (s == T(0)) return a;  // nothing in it
+  const T d = b.m - a.m, c = exp_below(d);
+  return {a.m, a.r + s * c, a.u + c * (b.u + s * d)};
 }
+
+// What one lane has read: its maximum m, s = sum e^(x - m) and u = sum e^(x - m) (x - m).
+template <typename T>
+struct Seen {
+  T m, s, u;
+};
 
 // N more values at a time: the maximum moves at most once, each value costs one exponential. A
 // value of -inf adds nothing (0 times the lowest value); NaN and +inf make s NaN.
 template <int N, typename T>
-__device__ __forceinline__ void push(Stats<T>& a, const T (&x)[N]) {
+__device__ __forceinline__ void push(Seen<T>& a, const T (&x)[N]) {
   T top = x[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) top = fmax(top, x[i]);
@@ -115,18 +127,9 @@ template <int LANES, typename T>
 __device__ __forceinline__ Stats<T> lanes_join(Stats<T> a) {
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1)
-    a = join(a, Stats<T>{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
+    a = join(a, Stats<T>{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.r, o),
                          __shfl_xor_sync(0xffffffffu, a.u, o)});
   return a;
-}
-
-template <typename T>
-__device__ __forceinline__ Stats<T> block_join(Stats<T> a, Stats<T>* sh) {
-  static_assert(kThreads / 32 == 8, "one lane of a group of eight to a warp");
-  a = lanes_join<32>(a);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = a;
-  __syncthreads();
-  return lanes_join<8>(sh[threadIdx.x & 7]);
 }
 
 template <typename T, int VE>
@@ -141,6 +144,10 @@ template <typename T>
 struct Shared {
   using U = typename OrderKey<T>::U;
   Stats<T> stats[kThreads / 32];
+  T tops_of[kThreads / 32];  // the warps' maxima
+  T rest[kThreads / 32];     // their shares of what the maximum's lane has read
+  int equal[kThreads / 32];
+  int holder;               // the first lane that has the maximum
   Stats<T> mine;            // the block's, for the cluster
   Alt<U> list[kList];       // candidates
   Alt<U> best[kMaxTop];     // the block's alternatives in order
@@ -252,6 +259,59 @@ __device__ void select_top(const T* __restrict__ x, int n, int first, int top_k,
   __syncthreads();
 }
 
+// The block's statistics from its lanes'. A lane's s holds its maximum's own 1, which rounds what
+// is small beside it away; that matters in the lane that holds the block's maximum alone, so the
+// block reads that lane's values (a kThreads-th of the row) once more and sums them without it.
+template <typename T, int VE>
+__device__ Stats<T> block_stats(Seen<T> a, const Vec<T, VE>* __restrict__ xv, int units,
+                                Shared<T>& sh) {
+  static_assert(kThreads / 32 == 8, "one lane of a group of eight to a warp");
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const T top = warp_max(a.m);
+  if (lane == 0) sh.tops_of[w] = top;
+  if (threadIdx.x == 0) sh.holder = kThreads;
+  __syncthreads();
+  T m = sh.tops_of[lane & 7];
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (a.m == m && a.s != T(0)) atomicMin(&sh.holder, (int)threadIdx.x);
+  __syncthreads();
+  const int holder = sh.holder;
+  T rest = T(0);
+  int equal = 0;  // entries equal to the maximum, one of them the maximum itself
+  if (holder < kThreads) {
+    for (int c = holder + threadIdx.x * kThreads; c < units; c += kThreads * kThreads) {
+      const Vec<T, VE> y = xv[c];
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        equal += y.v[e] == m;
+        rest += y.v[e] == m ? T(0) : exp_below(y.v[e] - m);
+      }
+    }
+  }
+  equal = __reduce_add_sync(0xffffffffu, equal);
+  rest = warp_sum(rest);
+  Stats<T> mine{a.m, a.s == T(0) ? T(-1) : a.s - T(1), a.u};
+  if ((int)threadIdx.x == holder && a.s == a.s) mine.r = T(0);
+  mine = lanes_join<32>(mine);
+  if (lane == 0) {
+    sh.stats[w] = mine;
+    sh.rest[w] = rest;
+    sh.equal[w] = equal;
+  }
+  __syncthreads();
+  mine = lanes_join<8>(sh.stats[lane & 7]);
+  rest = sh.rest[lane & 7];
+  equal = sh.equal[lane & 7];
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) {
+    rest += __shfl_xor_sync(0xffffffffu, rest, o);
+    equal += __shfl_xor_sync(0xffffffffu, equal, o);
+  }
+  if (holder < kThreads) mine.r += rest + (T)(equal - 1);
+  return mine;
+}
+
 template <typename T>
 struct ScoreArgs {
   const T* logits;
@@ -279,30 +339,40 @@ __device__ __forceinline__ T target_log_prob(const ScoreArgs<T>& a, int64_t r, c
   return (row[t] - m) - ls;
 }
 
-// A row's part of the VJP: dx_j = -p_j (g_log + sum g_top + g_ent (log p_j + H)), then g_log at the
-// target and g_top at the alternatives. Built by whole warps.
+// A row's part of the VJP: dx_j = direct_j - p_j (total + g_ent (log p_j + H)), with direct_j what
+// comes in at class j alone (g_log at the target, g_top at the alternatives) and total their sum.
+// Built by whole warps.
 template <typename T>
 struct Pull {
-  T m, inv, a, slope, log;  // -p (a + slope z) with z = x - m: log p + H = z + (H - log s)
-  int64_t target;           // -1 without one
-  __device__ Pull(int64_t r, int classes, const int64_t* targets, const T* stats,
+  T m, r, inv, total, shift, slope, log;  // shift = H - log s, slope = g_ent, log = g_log
+  int64_t target;                         // -1 without one
+  __device__ Pull(int64_t row, int classes, const int64_t* targets, const T* stats,
                   const T* entropy, const T* g_log, const T* g_ent, const T* g_top, int top_k,
                   int64_t ignore_index) {
-    m = stats[2 * r];
-    const T s = stats[2 * r + 1], ls = dev_log<T>(s);
-    inv = T(1) / s;
-    target = targets[r];
+    m = stats[2 * row];
+    r = stats[2 * row + 1];
+    inv = T(1) / (T(1) + r);
+    target = targets[row];
     if (target == ignore_index || target < 0 || target >= classes) target = -1;
-    log = target >= 0 && g_log ? g_log[r] : T(0);
-    slope = g_ent ? g_ent[r] : T(0);
+    log = target >= 0 && g_log ? g_log[row] : T(0);
+    slope = g_ent ? g_ent[row] : T(0);
+    shift = entropy[row] - log_1p(r);
     T tops = T(0);
-    for (int k = threadIdx.x & 31; k < top_k; k += 32) tops += g_top[r * top_k + k];
+    for (int k = threadIdx.x & 31; k < top_k; k += 32) tops += g_top[row * top_k + k];
     if (top_k > 0) tops = warp_sum(tops);
-    a = log + tops + slope * (entropy[r] - ls);
+    total = log + tops;
   }
+  // A class at which nothing comes in alone.
   __device__ __forceinline__ T spread(T x) const {
     const T z = x - m, p = exp_below(z) * inv;
-    return p == T(0) ? T(0) : -p * (a + slope * z);  // nothing is left where log p may be -inf
+    // Nothing is left where log p may be -inf.
+    return p == T(0) ? T(0) : -p * (total + slope * (z + shift));
+  }
+  // One at which `direct` does: direct (1 - p) - p (the rest), with 1 - p = r / (1 + r) at the
+  // maximum, so that a nearly certain token's gradient keeps its digits.
+  __device__ __forceinline__ T single(T x, T direct) const {
+    const T z = x - m, p = exp_below(z) * inv, q = z == T(0) ? r * inv : T(1) - p;
+    return direct * q - (p == T(0) ? T(0) : p * ((total - direct) + slope * (z + shift)));
   }
 };
 
@@ -322,7 +392,7 @@ scores_fwd_kernel(ScoreArgs<T> a) {
   const int n = a.classes - first < a.part ? a.classes - first : a.part;
   const T* row = a.logits + r * a.classes;
   const T* x = row + first;
-  Stats<T> mine{kLowest<T>, T(0), T(0)};
+  Seen<T> seen{kLowest<T>, T(0), T(0)};
   const int units = n / VE;  // parts are multiples of VE
   const Vec<T, VE>* xv = reinterpret_cast<const Vec<T, VE>*>(x);
   int c = threadIdx.x;
@@ -335,22 +405,21 @@ scores_fwd_kernel(ScoreArgs<T> a) {
 #pragma unroll
       for (int e = 0; e < VE; ++e) v[i * VE + e] = y.v[e];
     }
-    push(mine, v);
+    push(seen, v);
   }
   for (; c < units; c += kThreads) {
     const Vec<T, VE> y = xv[c];
-    push(mine, y.v);
+    push(seen, y.v);
   }
-  const T lane_top = mine.m;
-  mine = block_join(mine, sh.stats);
-  if (a.top_k > 0) select_top<T, VE>(x, n, first, a.top_k, lane_top, sh);
+  Stats<T> mine = block_stats<T, VE>(seen, xv, units, sh);
+  if (a.top_k > 0) select_top<T, VE>(x, n, first, a.top_k, seen.m, sh);
   if (a.splits > 1) {
     const auto cluster = cooperative_groups::this_cluster();
     if (threadIdx.x == 0) sh.mine = mine;
     cluster.sync();
     const int other = threadIdx.x & 7;
     mine = lanes_join<8>(other < a.splits ? *cluster.map_shared_rank(&sh.mine, other)
-                                          : Stats<T>{kLowest<T>, T(0), T(0)});
+                                          : no_stats<T>());
     if (split == 0) {
       for (int i = threadIdx.x; i < a.splits * a.top_k; i += kThreads)
         sh.list[i] = cluster.map_shared_rank(sh.best, i / a.top_k)[i % a.top_k];
@@ -358,8 +427,8 @@ scores_fwd_kernel(ScoreArgs<T> a) {
     cluster.sync();  // the others' results have been read
   }
   if (split != 0) return;
-  const T ls = dev_log<T>(mine.s);
-  const T m = mine.s != T(0) ? mine.m : T(-INFINITY);  // a closed row has no log probabilities
+  const T ls = log_1p(mine.r);
+  const T m = mine.r != T(-1) ? mine.m : T(-INFINITY);  // a closed row has no log probabilities
   auto place = [&](int rank, Alt<U> e) {
     a.top[r * a.top_k + rank] = (row[e.id] - m) - ls;
     a.ids[r * a.top_k + rank] = e.id;
@@ -371,8 +440,8 @@ scores_fwd_kernel(ScoreArgs<T> a) {
   }
   if (threadIdx.x == 0) {
     a.stats[2 * r] = m;
-    a.stats[2 * r + 1] = mine.s;
-    a.entropy[r] = ls - mine.u / mine.s;
+    a.stats[2 * r + 1] = mine.r;
+    a.entropy[r] = ls - mine.u / (T(1) + mine.r);
     a.log_probs[r] = target_log_prob(a, r, row, m, ls);
   }
 }
@@ -402,25 +471,25 @@ scores_bwd_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targ
     for (int e = 0; e < VE; ++e) v.v[e] = p.spread(v.v[e]);
     dv[c] = v;
   }
-  // The single classes, by one lane each: the alternatives are distinct, the target may be
+  // The single classes again, by one lane each: the alternatives are distinct, the target may be
   // one of them.
+  const T* x = logits + r * classes + first;
   bool hit = false;
-  const int64_t at = p.target - first;
+  const int64_t at = p.target >= 0 ? p.target - first : -1;
   __syncthreads();
   for (int k = threadIdx.x; k < top_k; k += kThreads) {
     const int64_t i = ids[r * top_k + k] - first;
     if (i < 0 || i >= n) continue;
-    const bool same = p.target >= 0 && i == at;
-    hit |= same;
-    d[i] += g_top[r * top_k + k] + (same ? p.log : T(0));
+    hit |= i == at;
+    d[i] = p.single(x[i], g_top[r * top_k + k] + (i == at ? p.log : T(0)));
   }
   hit = __syncthreads_or(hit);
-  if (threadIdx.x == 0 && p.target >= 0 && !hit && at >= 0 && at < n) d[at] += p.log;
+  if (threadIdx.x == 0 && !hit && at >= 0 && at < n) d[at] = p.single(x[at], p.log);
 }
 
 // Rows of up to kWarpRow classes: a warp a row, its values in registers (NV of them to a lane),
 // alternatives taken one by one. A block a row leaves most of its lanes idle there (8192 rows of 65
-// classes forward and backward: 42.5 us, with a warp a row 7.1).
+// classes forward and backward: 42.5 us, with a warp a row 8.1).
 constexpr int kWarpRow = 1024;
 
 template <typename T, int NV>
@@ -433,7 +502,7 @@ scores_fwd_warp_kernel(ScoreArgs<T> a, int64_t rows) {
   const int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   if (r >= rows) return;
   const T* row = a.logits + r * a.classes;
-  T v[NV], m = kLowest<T>, s = T(0), u = T(0);
+  T v[NV], m = kLowest<T>, rest = T(0), u = T(0);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = lane + 32 * i;
@@ -441,16 +510,23 @@ scores_fwd_warp_kernel(ScoreArgs<T> a, int64_t rows) {
     m = fmax(m, v[i]);
   }
   m = warp_max(m);
+  bool has = false;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) has |= v[i] == m;
+  const unsigned holders = __ballot_sync(0xffffffffu, has);
+  bool out = lane == __ffs(holders) - 1;  // this lane leaves the maximum's own 1 out, once
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const T z = v[i] - m, e = exp_below(z);
-    s += e;
+    const T z = v[i] - m, e = out && v[i] == m ? T(0) : exp_below(z);
+    out = out && v[i] != m;
+    rest += e;
     u += e * fmax(z, kLowest<T>);
   }
-  s = warp_sum(s);
+  rest = holders == 0 ? T(-1) : warp_sum(rest);
+  if (m == T(INFINITY)) rest = T(NAN);
   u = warp_sum(u);
-  const T ls = dev_log<T>(s);
-  if (s == T(0)) m = T(-INFINITY);  // a closed row has no log probabilities
+  const T ls = log_1p(rest);
+  if (rest == T(-1)) m = T(-INFINITY);  // a closed row has no log probabilities
   if (a.top_k > 0) {
     // Every lane offers its first entry that has not been taken; the one that wins looks for
     // its next.
@@ -485,8 +561,8 @@ scores_fwd_warp_kernel(ScoreArgs<T> a, int64_t rows) {
   }
   if (lane == 0) {
     a.stats[2 * r] = m;
-    a.stats[2 * r + 1] = s;
-    a.entropy[r] = ls - u / s;
+    a.stats[2 * r + 1] = rest;
+    a.entropy[r] = ls - u / (T(1) + rest);
     a.log_probs[r] = target_log_prob(a, r, row, m, ls);
   }
 }
@@ -508,12 +584,13 @@ scores_bwd_warp_kernel(const T* __restrict__ logits, const int64_t* __restrict__
   const T* x = logits + r * classes;
   T* d = grad + r * classes;
 #pragma unroll 8
-  for (int c = lane; c < classes; c += 32) {
-    const T g = p.spread(x[c]);
-    d[c] = c == p.target ? g + p.log : g;
-  }
+  for (int c = lane; c < classes; c += 32)
+    d[c] = c == p.target ? p.single(x[c], p.log) : p.spread(x[c]);
   __syncwarp();
-  for (int k = lane; k < top_k; k += 32) d[ids[r * top_k + k]] += g_top[r * top_k + k];
+  for (int k = lane; k < top_k; k += 32) {
+    const int64_t i = ids[r * top_k + k];
+    d[i] = p.single(x[i], g_top[r * top_k + k] + (i == p.target ? p.log : T(0)));
+  }
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -220,6 +220,41 @@ def test_gradients_against_differences():
     gradgradcheck(total, [x])
 
 
+@pytest.mark.parametrize("dtype", [np.float32, np.float64], ids=["fp32", "fp64"])
+@pytest.mark.parametrize("classes", [7, 130, 1000, 5000, 50304])
+def test_nearly_certain_tokens_keep_their_digits(classes, dtype):
+    """A class 15 to 25 above the others: log p and H are of the size of e^-15, far below a step
+    of 1. Relative error: every e^(x - m) is off by (4 + 2.4 |x - m|) h and one rounding of its
+    argument's |x - m| h, the sum of n to a lane by 12 (n + 16) h; log1p, the quotient and the
+    last addition of two positive terms by a few h. |x - m| is at most 40 here."""
+    import tensorgrad_b200 as tg
+
+    rng = np.random.default_rng(classes)
+    rows = 6
+    x = rng.standard_normal((rows, classes)).astype(dtype)
+    t = rng.integers(0, classes, rows)
+    x[np.arange(rows), t] += np.linspace(15, 25, rows).astype(dtype)
+    tx = tg.Tensor(x, requires_grad=True)
+    got = tg.token_log_probs(tx, t, top_k=2)
+    given, ent, top, _, p, lp = _definition(x, t, 2)
+    # Extended precision has digits to spare for the definition's own 1 - p and log.
+    z = x.astype(np.longdouble) - x.max(-1, keepdims=True)
+    e = np.exp(z)
+    e[np.arange(rows), t] = 0
+    rest = e.sum(-1)
+    lp_t = -np.log1p(rest)
+    ent = np.log1p(rest) - (e * z).sum(-1) / (1 + rest)
+    h = _half(dtype)
+    rel = (12 * (-(-classes // THREADS) + 16) + 2 * (4 + 3.4 * 40) + 8) * h
+    assert np.all(np.abs(got.log_probs.numpy() - lp_t) <= rel * np.abs(lp_t))
+    assert np.all(np.abs(got.top_log_probs.numpy()[:, 0] - lp_t) <= rel * np.abs(lp_t))
+    assert np.all(np.abs(got.entropy.numpy() - ent) <= rel * np.abs(ent))
+    tg.autograd.backward([got.log_probs], [np.ones(rows)])
+    want = rest / (1 + rest)  # 1 - p of the target
+    g = tx.grad.numpy()[np.arange(rows), t]
+    assert np.all(np.abs(g - want) <= rel * np.abs(want))
+
+
 def test_each_output_alone_and_used_twice():
     import tensorgrad_b200 as tg
 
