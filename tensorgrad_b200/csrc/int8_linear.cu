@@ -314,13 +314,16 @@ int8_tile_kernel(const int8_t* __restrict__ a, const int8_t* __restrict__ b, int
   }
 }
 
+// Shared memory for the rows' integers: what a launch has without asking, less 1 KB for the rest.
+constexpr int64_t kFewBytes = 47 * 1024;
+
 // Up to 8 rows take the one-launch kernel, more than 2 of them only below 16384 channels: there its
 // multiplications cost more than the tensor cores' second launch (8 rows of 4096 through 4096
 // channels 12.2 us against 15.5, 6 of 2048 through 8192 8.2 against 10.5, 8 of 768 through 50304
 // 23.2 against 16.9; 2 rows 11.4 against 16.4).
 bool takes_few(int64_t rows, int64_t inner, int64_t outer) {
   return rows <= 8 && (rows <= 2 || outer < 16384) &&
-         (rows > 4 ? 8 : (rows > 2 ? 4 : rows)) * padded(inner) <= 49152;
+         (rows > 4 ? 8 : (rows > 2 ? 4 : rows)) * padded(inner) <= kFewBytes;
 }
 
 template <typename T, int R, int CH, int NV>

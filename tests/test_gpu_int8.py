@@ -41,7 +41,8 @@ def _check(y, x, q, scale, bias):
 SHAPES = [(1, 1, 1), (1, 768, 2304), (7, 16, 1), (2, 17, 5), (8, 4096, 300), (9, 100, 70),
           (16, 768, 1000), (33, 1001, 77), (128, 64, 256), (129, 130, 65), (300, 4096, 513),
           (1, 8192, 40), (2000, 256, 640), (1025, 48, 2052), (64, 2000, 129), (257, 1024, 4096),
-          (16, 4096, 4100), (2100, 130, 4500), (2049, 2100, 4100), (600, 3000, 8195)]
+          (1, 48128, 5), (1, 49000, 3), (2, 24064, 4), (5, 6016, 9), (8, 6100, 7), (16, 4096, 4100),
+          (2100, 130, 4500), (2049, 2100, 4100), (600, 3000, 8195)]
 
 
 @pytest.mark.parametrize("rows,inner,outer", SHAPES)
