@@ -123,6 +123,8 @@ int tg_int8_tc_status(int reset);
  * first wait on a load runs out, TG_ERR_TIMEOUT is recorded and the kernel drains and
  * returns with nothing in flight. Synchronous. */
 int tg_attention_set_wait_test(int64_t budget_cycles, int withhold_loads);
+/* The same for the 8-bit integer products. */
+int tg_int8_set_wait_test(int64_t budget_cycles, int withhold_loads);
 /* Test support (no reference counterpart): y[i] = the fp32 exponential the fused attention
  * kernels compute on the FMA pipe for part of their softmax numerators (range reduction plus
  * a fitted polynomial; see csrc/expfma.cuh), so a test can bound its error. */

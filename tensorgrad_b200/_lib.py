@@ -94,6 +94,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tg_attention_tc_status": (c_int, [c_int]),
     "tg_int8_tc_status": (c_int, [c_int]),
     "tg_attention_set_wait_test": (c_int, [i64, c_int]),
+    "tg_int8_set_wait_test": (c_int, [i64, c_int]),
     "tg_test_exp_fma": (c_int, [i64, vp, vp, vp]),
     "tg_set_matmul_precision": (c_int, [c_int]),
     "tg_gemm_profile": (c_int, [c_int]),

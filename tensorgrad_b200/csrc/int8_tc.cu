@@ -28,6 +28,10 @@ constexpr int kI8Epi0 = 4, kI8EpiWarps = 8;
 constexpr uint32_t kI8Box = 32 * 32 * 4;
 constexpr int kGroupM = 16;  // row tiles that share their column tiles' loads through the L2
 
+// Set only by tg_int8_set_wait_test: the producers then issue no load, so the first wait for one
+// runs out and the kernel's abort-and-drain path runs with nothing in flight.
+__device__ int g_withhold_loads = 0;
+
 template <int BN, bool PAIR>
 struct I8Layout {
   static constexpr int TILE_M = PAIR ? 256 : 128;
@@ -162,7 +166,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   if (warp == 0) {
     if (lane == 0) {
       int it = 0;
-      bool stop = false;
+      bool stop = *(volatile int*)&g_withhold_loads != 0;
       for (int t = unit; t < tiles && !stop; t += units) {
         int m, n;
         i8_tile(a, t, m, n);
@@ -437,4 +441,15 @@ extern "C" int tg_int8_tc_status(int reset) {
     cudaMemcpyToSymbol(tg::tc::g_status, &z, sizeof(int));
   }
   return v;
+}
+
+// Test support for these bounded waits (no reference counterpart): a wait budget in clock cycles
+// (<= 0 restores the default of about two seconds) and, with withhold_loads != 0, producers that
+// issue no load. Synchronous; affects later launches of this unit's kernels only.
+extern "C" int tg_int8_set_wait_test(int64_t budget_cycles, int withhold_loads) {
+  const long long b = budget_cycles > 0 ? (long long)budget_cycles : tg::tc::kTimeoutCycles;
+  const int w = withhold_loads ? 1 : 0;
+  TG_CUDA_TRY(cudaMemcpyToSymbol(tg::tc::g_wait_budget, &b, sizeof(b)));
+  TG_CUDA_TRY(cudaMemcpyToSymbol(tg::tc::g_withhold_loads, &w, sizeof(w)));
+  return TG_OK;
 }

@@ -183,3 +183,30 @@ def test_int8_layer_is_the_operator():
         small(tg.Tensor(x, requires_grad=True))
     with tg.no_grad():
         small(tg.Tensor(x, requires_grad=True))
+
+
+@pytest.mark.parametrize("rows,inner,outer", [(300, 256, 700), (2049, 2100, 4100)])
+def test_wait_that_runs_out_reports_and_recovers(rows, inner, outer):
+    """The bounded waits of the tensor-core product (one CTA to a tile, and a pair): with no
+    load issued and a budget of about a millisecond the first wait gives up, the kernel drains
+    with nothing in flight, and the next synchronisation raises; afterwards the same call is
+    right again."""
+    import tensorgrad_b200 as tg
+    from tensorgrad_b200 import device
+    from tensorgrad_b200._lib import check, lib
+
+    rng = np.random.default_rng(rows)
+    x = rng.standard_normal((rows, inner)).astype(np.float32)
+    w = rng.standard_normal((outer, inner)).astype(np.float32)
+    weight, tx = tg.Int8Weight.quantize(tg.Tensor(w)), tg.Tensor(x)
+    device.synchronize()
+    check(lib.tg_int8_set_wait_test(2_000_000, 1))
+    try:
+        y = tg.int8_linear(tx, weight)
+        with pytest.raises(RuntimeError, match="8-bit integer linear: a bounded device-side wait"):
+            device.synchronize()
+        del y
+    finally:
+        check(lib.tg_int8_set_wait_test(0, 0))
+    device.synchronize()
+    _check(tg.int8_linear(tx, weight).numpy(), x, *_quantized(w), None)
