@@ -379,7 +379,7 @@ struct Pull {
 // One block a row, or a cluster of `splits` blocks with a part of its classes each. HBM-bound: one
 // read of the logits, VE of them to a load; 8 instructions and one exponential a value.
 template <typename T, int VE>
-__global__ void __launch_bounds__(kThreads, 4)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 5 : 4)
 scores_fwd_kernel(ScoreArgs<T> a) {
   using U = typename OrderKey<T>::U;
   constexpr int N = 4;  // loads in a step
@@ -487,9 +487,10 @@ scores_bwd_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targ
   if (threadIdx.x == 0 && !hit && at >= 0 && at < n) d[at] = p.single(x[at], p.log);
 }
 
-// Rows of up to kWarpRow classes: a warp a row, its values in registers (NV of them to a lane),
-// alternatives taken one by one. A block a row leaves most of its lanes idle there (8192 rows of 65
-// classes forward and backward: 42.5 us, with a warp a row 8.1).
+// Rows of up to kWarpRow classes: a warp a row, its values in registers (NV of them to a lane). A
+// block a row leaves most of its lanes idle there (8192 rows of 65 classes forward and backward:
+// 42.5 us, with a warp a row 8.1). Alternatives by bisecting their keys cost the same for any
+// number of them (8192 x 1000: 5 of them 57 us, 100 of them 88; one by one 54 and 601).
 constexpr int kWarpRow = 1024;
 
 template <typename T, int NV>
@@ -528,35 +529,45 @@ scores_fwd_warp_kernel(ScoreArgs<T> a, int64_t rows) {
   const T ls = log_1p(rest);
   if (rest == T(-1)) m = T(-INFINITY);  // a closed row has no log probabilities
   if (a.top_k > 0) {
-    // Every lane offers its first entry that has not been taken; the one that wins looks for
-    // its next.
-    uint32_t taken = 0;
-    Alt<U> mine;
-    auto offer = [&] {
-      mine = {0, std::numeric_limits<int>::max()};
+    // The top_k-th key, bit by bit: the largest that at least top_k entries reach. Entries above
+    // it and the first ones equal to it are the alternatives; their order is by rank.
+    U key[NV], kth = 0;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = lane + 32 * i;
-        const Alt<U> e{OrderKey<T>::of(v[i]), c};
-        if (c < a.classes && !(taken >> i & 1) && before(e, mine)) mine = e;
-      }
-    };
-    offer();
-    for (int k = 0; k < a.top_k; ++k) {
-      Alt<U> best = mine;
+    for (int i = 0; i < NV; ++i) key[i] = OrderKey<T>::of(v[i]);
+    for (int bit = 8 * (int)sizeof(U) - 1; bit >= 0; --bit) {
+      const U next = kth | (U)1 << bit;
+      int reach = 0;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const Alt<U> other{__shfl_xor_sync(0xffffffffu, best.key, o),
-                           __shfl_xor_sync(0xffffffffu, best.id, o)};
-        if (before(other, best)) best = other;
-      }
-      if (best.id % 32 == lane) {
-        a.top[r * a.top_k + k] = (row[best.id] - m) - ls;
-        a.ids[r * a.top_k + k] = best.id;
-        taken |= 1u << (best.id / 32);
-        offer();
-      }
-      __syncwarp();
+      for (int i = 0; i < NV; ++i) reach += lane + 32 * i < a.classes && key[i] >= next;
+      if (__reduce_add_sync(0xffffffffu, reach) >= a.top_k) kth = next;
+    }
+    __shared__ Alt<U> lists[kThreads / 32][kMaxTop];
+    Alt<U>* list = lists[threadIdx.x >> 5];
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) above += lane + 32 * i < a.classes && key[i] > kth;
+    int ties = __reduce_add_sync(0xffffffffu, above);
+    above = 0;
+    const unsigned before_me = (1u << lane) - 1;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const bool in = lane + 32 * i < a.classes;
+      const unsigned more = __ballot_sync(0xffffffffu, in && key[i] > kth);
+      const unsigned same = __ballot_sync(0xffffffffu, in && key[i] == kth);
+      if (more >> lane & 1) list[above + __popc(more & before_me)] = {key[i], lane + 32 * i};
+      const int at = ties + __popc(same & before_me);
+      if ((same >> lane & 1) && at < a.top_k) list[at] = {key[i], lane + 32 * i};
+      above += __popc(more);
+      ties += __popc(same);
+    }
+    __syncwarp();
+    for (int k = lane; k < a.top_k; k += 32) {
+      const Alt<U> mine = list[k];
+      int rank = 0;
+#pragma unroll 4
+      for (int j = 0; j < a.top_k; ++j) rank += before(list[j], mine);
+      a.top[r * a.top_k + rank] = (row[mine.id] - m) - ls;
+      a.ids[r * a.top_k + rank] = mine.id;
     }
   }
   if (lane == 0) {
