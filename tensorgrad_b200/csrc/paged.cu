@@ -815,8 +815,10 @@ int check_pool(const char* what, int64_t num_pages, int64_t kv_heads, int64_t pa
 // The rows of (batch, heads, positions), and how many blocks of LPR lanes a row they make.
 int make_moves(const char* what, const Pool& pool, int64_t batch, int64_t positions,
                const int64_t* lengths, Moves& m) {
-  TG_CHECK_ARG(batch <= INT32_MAX / pool.kv_heads / positions, "%s: %lld x %lld x %lld rows", what,
-               (long long)batch, (long long)pool.kv_heads, (long long)positions);
+  // Half the range: a lane's next row is worked out before it is compared.
+  TG_CHECK_ARG(batch <= INT32_MAX / 2 / pool.kv_heads / positions,
+               "%s: %lld x %lld x %lld rows", what, (long long)batch, (long long)pool.kv_heads,
+               (long long)positions);
   m.pool = pool;
   m.rows = (int)(batch * pool.kv_heads * positions);
   m.heads = make_div(pool.kv_heads);

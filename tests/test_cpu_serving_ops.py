@@ -153,6 +153,10 @@ def test_page_entry_points_refuse_bad_sizes():
     assert lib.tg_page_copy_few(8, 1, 4, None, None, at + 8, at, 1, None) == 4
     assert lib.tg_page_copy_few(8, 1, 4, None, None, None, None, 65, None) == 1
     assert lib.tg_page_copy_few(8, 1, 4, None, None, None, None, 0, None) == 0
+    assert lib.tg_paged_gather(0, 1 << 10, 1 << 20, 1, 1, None, None, 1, 1 << 20, None, 1, None,
+                               None, None, None, None) == 1
+    assert lib.tg_paged_gather(0, 1, 1, 1, 1, None, None, 1, 1 << 20, None, 1 << 11, None, None,
+                               None, None, None) == 1
     assert lib.tg_paged_gather(0, 1, -1, 1, 1, None, None, 1, 1, None, 1, None, None, None, None,
                                None) == 1
 
