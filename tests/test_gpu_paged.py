@@ -109,6 +109,29 @@ def test_attention_matches_definition(lengths, heads, kv_heads, width, size, dty
     assert np.all(np.abs(lse.numpy()[full] - ref_lse[full]) <= 2 * scale)
 
 
+@pytest.mark.parametrize("heads,kv_heads,width", [(1, 1, 64), (8, 2, 128), (8, 1, 40)])
+@pytest.mark.parametrize("course", ["rises", "falls", "creeps", "leaps"])
+def test_attention_where_the_maximum_moves(course, heads, kv_heads, width, dtype):
+    """Scores that climb or fall by tens, by less than one in all, or in steps of some hundred."""
+    import tensorgrad_b200 as tg
+
+    rng = np.random.default_rng(width)
+    keys, values, table, held = _cache(rng, dtype, [900, 70], kv_heads, width, 16)
+    u = rng.choice([-1.0, 1.0], width)
+    t = np.linspace(0, 1, 900)
+    reach = {"rises": 60 * t, "falls": 60 * (1 - t), "creeps": t,
+             "leaps": 150 * np.floor(5 * t)}[course]
+    for b, n in enumerate(held):
+        for at in range(n):
+            row = keys[table[b, at // 16], :, at % 16]
+            row *= 0.25
+            row += (reach[at] / np.sqrt(width) * u).astype(dtype)
+    q = (u + 0.25 * rng.standard_normal((2, heads, width))).astype(dtype)
+    out = tg.paged_attention(tg.Tensor(q), tg.Tensor(keys), tg.Tensor(values), table, held)
+    ref, _, bound = _attention(q, keys, values, table, held)
+    assert np.all(np.abs(out.numpy() - ref) <= bound * np.finfo(dtype).eps / 2)
+
+
 def test_device_tables_hints_and_views_give_the_same(dtype):
     import tensorgrad_b200 as tg
     from tensorgrad_b200 import device
