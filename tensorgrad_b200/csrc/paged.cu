@@ -343,8 +343,8 @@ __device__ __forceinline__ int split_length(int n, int splits) {
 // The U GH scores of a group are reduced by halving: at each of the first levels a lane keeps
 // half of its partial scores and hands the other half over, so that a score is finished, and its
 // exponential taken, in one lane (LPT / (U GH) lanes), and is then dealt out to the group.
-// What bounds it: reading keys and values once; behind that the issue slots (at 4 heads of 128 to
-// a key head they are two thirds taken).
+// What bounds it: reading keys and values once (6.5 to 6.8 TB/s up to 4 heads of 128 to a key
+// head), behind that the issue slots (8 heads: 4.9 TB/s).
 constexpr int U = 2;
 
 // The maximum that weights are taken against follows only when a score is above it by more than
@@ -457,16 +457,28 @@ paged_attention_kernel(AttendArgs a, const T* __restrict__ q, const T* __restric
     }
     __syncthreads();
     const int steps = (t1 - t0 + STEP - 1) / STEP;
+    // Each lane of a group looks up the group's positions of one of the next LPT rounds, and hands
+    // them out when their round comes: in every lane for every round it was a sixth of all
+    // instructions (8 heads of 128 to a key head, 4 x 8 of them up to 65536 positions: 345 -> 315
+    // us; the double case above: 137 -> 128 us).
+    int64_t where[U];
     auto issue = [&](int i) {
+      if (i % LPT == 0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int t = t0 + (i + j) * STEP + u * ROWS + my_row;
+          where[u] = -1;
+          if (t < t1) {
+            const int p = div_by(t, a.size);
+            where[u] = table[p - p0] + (int64_t)(t - p * (int)a.size.d) * d;
+          }
+        }
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int t = t0 + i * STEP + u * ROWS + my_row;
-        const bool live = t < t1;
-        int64_t at = j * VE;
-        if (live) {
-          const int p = div_by(t, a.size);
-          at += table[p - p0] + (int64_t)(t - p * (int)a.size.d) * d;
-        }
+        const int64_t row = __shfl_sync(0xffffffffu, where[u], sub * LPT + i % LPT);
+        const bool live = row >= 0;
+        const int64_t at = (live ? row : 0) + j * VE;
         const uint32_t to = ring + (i % ST) * A::STAGE + u * A::ROW;
         const T* k = keys + at;
         const T* v = values + at;
@@ -727,7 +739,8 @@ int sm_count() {
 // Query heads that one block takes: the group of a key head, rounded up to a power of two, at
 // most 4 (2 where the lanes hold double): 8 leave half as many warps for the registers, and two
 // blocks that share keys and values through the L2 are faster (8 heads of 64 to a key head, 64 x 4
-// of them up to 4096 positions: 190 us with 8, 116 with 4 a block).
+// of them up to 4096 positions: 190 us with 8, 116 with 4 a block; 96 since positions are looked up
+// once for many rounds).
 int heads_per_block(int dtype, int64_t group) {
   const int most = dtype == TG_F64 ? 2 : 4;
   int g = 1;
