@@ -81,7 +81,9 @@ __device__ __forceinline__ float log_1p(float x) { return log1pf(x); }
 __device__ __forceinline__ double log_1p(double x) { return log1p(x); }
 
 // The statistics of two sets of values as one: the lower maximum's set is scaled by
-// c = e^(its m - the other m), every x - m of it moves by the difference.
+// c = e^(its m - the other m), every x - m of it moves by the difference d. A set so low that c is
+// 0 (classes closed by the type's lowest value, say) adds nothing: its sum is scaled before d
+// multiplies it, as sum times d may overflow, and d itself is kept finite.
 template <typename T>
 __device__ __forceinline__ Stats<T> join(Stats<T> a, Stats<T> b) {
   if (b.m > a.m) {
@@ -91,8 +93,8 @@ __device__ __forceinline__ Stats<T> join(Stats<T> a, Stats<T> b) {
   }
   const T s = T(1) + b.r;
   if (s == T(0)) return a;  // nothing in it
-  const T d = b.m - a.m, c = exp_below(d);
-  return {a.m, a.r + s * c, a.u + c * (b.u + s * d)};
+  const T d = fmax(b.m - a.m, kLowest<T>), c = exp_below(d), moved = s * c;
+  return {a.m, a.r + moved, a.u + (c * b.u + moved * d)};
 }
 
 // What one lane has read: its maximum m, s = sum e^(x - m) and u = sum e^(x - m) (x - m).
@@ -109,9 +111,9 @@ __device__ __forceinline__ void push(Seen<T>& a, const T (&x)[N]) {
 #pragma unroll
   for (int i = 1; i < N; ++i) top = fmax(top, x[i]);
   if (top > a.m) {
-    const T d = a.m - top, c = exp_below(d);
-    a.u = a.s != T(0) ? c * (a.u + a.s * d) : T(0);
+    const T d = fmax(a.m - top, kLowest<T>), c = exp_below(d);
     a.s *= c;
+    a.u = c * a.u + a.s * d;  // finite as in join
     a.m = top;
   }
 #pragma unroll
@@ -356,7 +358,7 @@ struct Pull {
     if (target == ignore_index || target < 0 || target >= classes) target = -1;
     log = target >= 0 && g_log ? g_log[row] : T(0);
     slope = g_ent ? g_ent[row] : T(0);
-    shift = entropy[row] - log_1p(r);
+    shift = g_ent ? entropy[row] - log_1p(r) : T(0);
     T tops = T(0);
     for (int k = threadIdx.x & 31; k < top_k; k += 32) tops += g_top[row * top_k + k];
     if (top_k > 0) tops = warp_sum(tops);
