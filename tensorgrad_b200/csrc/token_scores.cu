@@ -73,10 +73,10 @@ __device__ __forceinline__ Stats<T> no_stats() {
   return {kLowest<T>, T(-1), T(0)};
 }
 
-// e^x for x <= 0. The float form multiplies by log2 e in the argument: off by (4 + 2.4 |x|) half
-// steps, and a term of size |x| weighs e^x.
-__device__ __forceinline__ float exp_below(float x) { return __expf(x); }
-__device__ __forceinline__ double exp_below(double x) { return exp(x); }
+// Exponentials are dev_exp's, a step off or two: an argument in base 2 (__expf) would be off by
+// (4 + 2.4 |x|) half steps, which is all that a low class's gradient or many equal low classes keep
+// of it (8192 x 50304 forward 260 -> 263 us, with the gradient 780 -> 791; 8192 x 1000 with 5
+// alternatives 62 -> 68).
 __device__ __forceinline__ float log_1p(float x) { return log1pf(x); }
 __device__ __forceinline__ double log_1p(double x) { return log1p(x); }
 
@@ -93,7 +93,7 @@ __device__ __forceinline__ Stats<T> join(Stats<T> a, Stats<T> b) {
   }
   const T s = T(1) + b.r;
   if (s == T(0)) return a;  // nothing in it
-  const T d = fmax(b.m - a.m, kLowest<T>), c = exp_below(d), moved = s * c;
+  const T d = fmax(b.m - a.m, kLowest<T>), c = dev_exp(d), moved = s * c;
   return {a.m, a.r + moved, a.u + (c * b.u + moved * d)};
 }
 
@@ -111,14 +111,14 @@ __device__ __forceinline__ void push(Seen<T>& a, const T (&x)[N]) {
 #pragma unroll
   for (int i = 1; i < N; ++i) top = fmax(top, x[i]);
   if (top > a.m) {
-    const T d = fmax(a.m - top, kLowest<T>), c = exp_below(d);
+    const T d = fmax(a.m - top, kLowest<T>), c = dev_exp(d);
     a.s *= c;
     a.u = c * a.u + a.s * d;  // finite as in join
     a.m = top;
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const T z = x[i] - a.m, e = exp_below(z);
+    const T z = x[i] - a.m, e = dev_exp(z);
     a.s += e;
     a.u += e * fmax(z, kLowest<T>);
   }
@@ -287,7 +287,7 @@ __device__ Stats<T> block_stats(Seen<T> a, const Vec<T, VE>* __restrict__ xv, in
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
         equal += y.v[e] == m;
-        rest += y.v[e] == m ? T(0) : exp_below(y.v[e] - m);
+        rest += y.v[e] == m ? T(0) : dev_exp(y.v[e] - m);
       }
     }
   }
@@ -366,14 +366,14 @@ struct Pull {
   }
   // A class at which nothing comes in alone.
   __device__ __forceinline__ T spread(T x) const {
-    const T z = x - m, p = exp_below(z) * inv;
+    const T z = x - m, p = dev_exp(z) * inv;
     // Nothing is left where log p may be -inf.
     return p == T(0) ? T(0) : -p * (total + slope * (z + shift));
   }
   // One at which `direct` does: direct (1 - p) - p (the rest), with 1 - p = r / (1 + r) at the
   // maximum, so that a nearly certain token's gradient keeps its digits.
   __device__ __forceinline__ T single(T x, T direct) const {
-    const T z = x - m, p = exp_below(z) * inv, q = z == T(0) ? r * inv : T(1) - p;
+    const T z = x - m, p = dev_exp(z) * inv, q = z == T(0) ? r * inv : T(1) - p;
     return direct * q - (p == T(0) ? T(0) : p * ((total - direct) + slope * (z + shift)));
   }
 };
@@ -520,7 +520,7 @@ scores_fwd_warp_kernel(ScoreArgs<T> a, int64_t rows) {
   bool out = lane == __ffs(holders) - 1;  // this lane leaves the maximum's own 1 out, once
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const T z = v[i] - m, e = out && v[i] == m ? T(0) : exp_below(z);
+    const T z = v[i] - m, e = out && v[i] == m ? T(0) : dev_exp(z);
     out = out && v[i] != m;
     rest += e;
     u += e * fmax(z, kLowest<T>);
