@@ -336,15 +336,17 @@ def _scores_composite(tl: Tensor, tgt: DeviceArray, ids: DeviceArray | None, row
     from tensorgrad_b200.ops.elementwise import exp, mul, neg
     from tensorgrad_b200.ops.shape import concat, getitem, masked_fill, reshape
 
-    x = reshape(tl, (rows, classes))
-    lp = masked_fill(log_softmax(x, -1), np.isneginf(x.numpy()), 0.0)
-    # A closed class is left out of the entropy by p log p = 0.
-    p = masked_fill(exp(lp), np.isneginf(x.numpy()), 0.0)
+    lp = log_softmax(reshape(tl, (rows, classes)), -1)
+    # A class without probability is left out of the entropy alone, by p log p = 0; as a target
+    # or an alternative its log probability has the gradient of any other's.
+    p = exp(lp)
+    none = p.numpy() == 0
+    p_log_p = mul(masked_fill(p, none, 0.0), masked_fill(lp, none, 0.0))
     t = tgt.numpy().reshape(-1)
     kept = (t != ignore_index) & (t >= 0) & (t < classes)
     at = np.arange(rows)
-    given = mul(getitem(lp, (at, np.where(kept, t, 0))), Tensor(kept.astype(lp.dtype)))
-    parts = [given, neg(reduce.sum(mul(p, lp), axis=-1))]
+    given = masked_fill(getitem(lp, (at, np.where(kept, t, 0))), ~kept, 0.0)
+    parts = [given, neg(reduce.sum(p_log_p, axis=-1))]
     if ids is not None:
         alt = ids.numpy().reshape(rows, top_k)
         parts.append(reshape(getitem(lp, (at[:, None], alt)), (rows * top_k,)))
