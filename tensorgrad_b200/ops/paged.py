@@ -62,6 +62,9 @@ def _table(what: str, pages: Any, lengths: Any, batch: int, num_pages: int, page
             raise TypeError(f"{what}: {name} must be integers, got {x.dtype}")
         if isinstance(x, DeviceArray) and x.dtype != np.int64:
             raise TypeError(f"{what}: {name} on the device must be int64, got {x.dtype}")
+    # As int64 before any arithmetic: lengths of a narrow type could wrap when `extra` is added.
+    table, held = (x.astype(np.int64, copy=False) if isinstance(x, np.ndarray) else x
+                   for x in (table, held))
     if len(table.shape) != 2 or table.shape[0] != batch or table.shape[1] == 0:
         raise ValueError(f"{what}: expected pages ({batch}, max_pages), got {table.shape}")
     if tuple(held.shape) != (batch,):
@@ -77,8 +80,8 @@ def _table(what: str, pages: Any, lengths: Any, batch: int, num_pages: int, page
             if ids.size and (ids.min() < 0 or ids.max() >= num_pages):
                 raise IndexError(f"{what}: page ids must be in [0, {num_pages})")
     checked = isinstance(table, np.ndarray) and isinstance(held, np.ndarray)
-    out = [device.from_numpy(np.ascontiguousarray(x, dtype=np.int64))
-           if isinstance(x, np.ndarray) else x for x in (table, held)]
+    out = [device.from_numpy(np.ascontiguousarray(x)) if isinstance(x, np.ndarray) else x
+           for x in (table, held)]
     bad = None if checked else device.async_error_word(device.ASYNC_CACHE_PAGE)
     return out[0], out[1], bad
 
