@@ -135,8 +135,8 @@ ASYNC_CLASS_TARGET = 1
 ASYNC_CACHE_PAGE = 2
 _ASYNC_MESSAGES = {
     ASYNC_EMBEDDING_ID: "embedding ids out of range (device-resident ids, checked on the device)",
-    ASYNC_CLASS_TARGET: "cross_entropy target out of range (device-resident targets, checked on "
-                        "the device)",
+    ASYNC_CLASS_TARGET: "class target out of range (device-resident targets of cross_entropy or "
+                        "token_log_probs, checked on the device)",
     ASYNC_CACHE_PAGE: "page ids or lengths outside the paged cache (device-resident, checked on "
                       "the device)",
 }
