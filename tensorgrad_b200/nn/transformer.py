@@ -229,6 +229,8 @@ class GPT(Module):
             raise ValueError("temperature must be positive")
         if samples < 1 or max_new_tokens < 0:
             raise ValueError(f"cannot draw {samples} samples of {max_new_tokens} tokens")
+        if page_size < 1:
+            raise ValueError(f"page_size must be positive, got {page_size}")
         texts = [np.asarray(p, dtype=np.int64) for p in prompts]
         for p in texts:
             if p.ndim != 1 or p.size == 0:
