@@ -273,9 +273,11 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads)
 int8_tile_kernel(const int8_t* __restrict__ a, const int8_t* __restrict__ b, int64_t ld,
                  int64_t b_ld, const T* __restrict__ a_scale, const T* __restrict__ b_scale,
-                 const T* __restrict__ bias, T* __restrict__ y, int64_t rows, int64_t outer) {
+                 const T* __restrict__ bias, T* __restrict__ y, int64_t rows, int64_t outer,
+                 unsigned tiles_n) {
   __shared__ int as[64][17], bs[64][17];
-  const int64_t m0 = (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
+  const int64_t m0 = (int64_t)(blockIdx.x / tiles_n) * 64;
+  const int64_t n0 = (int64_t)(blockIdx.x % tiles_n) * 64;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   int acc[4][4] = {};
   const int lr = threadIdx.x >> 2, lc = (threadIdx.x & 3) * 4;  // this thread's 16 bytes
@@ -443,11 +445,13 @@ int tg_int8_linear(int dtype, const void* x, int64_t rows, int64_t inner, const 
     return int8_gemm_tc(q, weight, ld, (const float*)after, (const float*)scales,
                         (const float*)bias, (float*)y, rows, inner, outer, s);
   return TG_DISPATCH_FLOAT(dtype, T, [&] {
-    TG_CHECK_ARG((rows + 63) / 64 <= 65535, "int8_linear: too many rows");
-    const dim3 grid((unsigned)((outer + 63) / 64), (unsigned)((rows + 63) / 64));
-    int8_tile_kernel<T><<<grid, kThreads, 0, s>>>(q, weight, k, ld, (const T*)after,
-                                                  (const T*)scales, (const T*)bias, (T*)y, rows,
-                                                  outer);
+    const int64_t tiles_n = (outer + 63) / 64, tiles_m = (rows + 63) / 64;
+    if (tiles_n > INT32_MAX / tiles_m)  // one axis of tiles: a grid's second one ends at 65535
+      return set_error(TG_ERR_UNSUPPORTED, "int8_linear: %lld x %lld outputs", (long long)rows,
+                       (long long)outer);
+    int8_tile_kernel<T><<<dim3((unsigned)(tiles_m * tiles_n)), kThreads, 0, s>>>(
+        q, weight, k, ld, (const T*)after, (const T*)scales, (const T*)bias, (T*)y, rows, outer,
+        (unsigned)tiles_n);
     return check_launch("int8_linear");
   });
 }
