@@ -73,10 +73,14 @@ __device__ __forceinline__ Stats<T> no_stats() {
   return {kLowest<T>, T(-1), T(0)};
 }
 
-// Exponentials are dev_exp's, a step off or two: an argument in base 2 (__expf) would be off by
-// (4 + 2.4 |x|) half steps, which is all that a low class's gradient or many equal low classes keep
-// of it (8192 x 50304 forward 260 -> 263 us, with the gradient 780 -> 791; 8192 x 1000 with 5
-// alternatives 62 -> 68).
+// Exponentials are dev_exp's, a step off or two, except in a lane's own sums (push): there the
+// argument is in base 2, off by (4 + 2.4 |x|) half steps. Its x is below that lane's own maximum,
+// whose term is an exact 1, so of n values a lane's sum is off by about 4 + 3.4 log n half steps at
+// most; whatever lies far below the row's maximum is moved there by one exact exponential a lane.
+// 8192 x 50304 forward and backward: 801 us, with dev_exp there too 814; with base 2 everywhere 796,
+// and a class 80 below the maximum off by 61 half steps.
+__device__ __forceinline__ float lane_exp(float x) { return __expf(x); }
+__device__ __forceinline__ double lane_exp(double x) { return exp(x); }
 __device__ __forceinline__ float log_1p(float x) { return log1pf(x); }
 __device__ __forceinline__ double log_1p(double x) { return log1p(x); }
 
@@ -118,7 +122,7 @@ __device__ __forceinline__ void push(Seen<T>& a, const T (&x)[N]) {
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const T z = x[i] - a.m, e = dev_exp(z);
+    const T z = x[i] - a.m, e = lane_exp(z);
     a.s += e;
     a.u += e * fmax(z, kLowest<T>);
   }
@@ -492,7 +496,7 @@ scores_bwd_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targ
 // Rows of up to kWarpRow classes: a warp a row, its values in registers (NV of them to a lane). A
 // block a row leaves most of its lanes idle there (8192 rows of 65 classes forward and backward:
 // 42.5 us, with a warp a row 8.1). Alternatives by bisecting their keys cost the same for any
-// number of them (8192 x 1000: 5 of them 57 us, 100 of them 88; one by one 54 and 601).
+// number of them (8192 x 1000: 5 of them 59 us, 100 of them 90; one by one about 54 and 600).
 constexpr int kWarpRow = 1024;
 
 template <typename T, int NV>
