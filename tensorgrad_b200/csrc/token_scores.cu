@@ -151,7 +151,8 @@ struct Shared {
   using U = typename OrderKey<T>::U;
   Stats<T> stats[kThreads / 32];
   T tops_of[kThreads / 32];  // the warps' maxima
-  T rest[kThreads / 32];     // their shares of what the maximum's lane has read
+  T rest[kThreads / 32];     // their shares of what the maximum's lane has read: the terms
+  T rest_u[kThreads / 32];   // beside the maximum's own, and those times x - m
   int equal[kThreads / 32];
   int holder;               // the first lane that has the maximum
   Stats<T> mine;            // the block's, for the cluster
@@ -267,7 +268,8 @@ __device__ void select_top(const T* __restrict__ x, int n, int first, int top_k,
 
 // The block's statistics from its lanes'. A lane's s holds its maximum's own 1, which rounds what
 // is small beside it away; that matters in the lane that holds the block's maximum alone, so the
-// block reads that lane's values (a kThreads-th of the row) once more and sums them without it.
+// block reads that lane's values (a kThreads-th of the row) once more and sums them without it,
+// with full exponentials: beside the maximum they may all be far below it.
 template <typename T, int VE>
 __device__ Stats<T> block_stats(Seen<T> a, const Vec<T, VE>* __restrict__ xv, int units,
                                 Shared<T>& sh) {
@@ -283,38 +285,47 @@ __device__ Stats<T> block_stats(Seen<T> a, const Vec<T, VE>* __restrict__ xv, in
   if (a.m == m && a.s != T(0)) atomicMin(&sh.holder, (int)threadIdx.x);
   __syncthreads();
   const int holder = sh.holder;
-  T rest = T(0);
+  T rest = T(0), rest_u = T(0);
   int equal = 0;  // entries equal to the maximum, one of them the maximum itself
   if (holder < kThreads) {
     for (int c = holder + threadIdx.x * kThreads; c < units; c += kThreads * kThreads) {
       const Vec<T, VE> y = xv[c];
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
+        const T z = y.v[e] - m, t = y.v[e] == m ? T(0) : dev_exp(z);
         equal += y.v[e] == m;
-        rest += y.v[e] == m ? T(0) : dev_exp(y.v[e] - m);
+        rest += t;
+        rest_u += t * fmax(z, kLowest<T>);
       }
     }
   }
   equal = __reduce_add_sync(0xffffffffu, equal);
   rest = warp_sum(rest);
+  rest_u = warp_sum(rest_u);
   Stats<T> mine{a.m, a.s == T(0) ? T(-1) : a.s - T(1), a.u};
-  if ((int)threadIdx.x == holder && a.s == a.s) mine.r = T(0);
+  if ((int)threadIdx.x == holder && a.s == a.s) mine.r = mine.u = T(0);
   mine = lanes_join<32>(mine);
   if (lane == 0) {
     sh.stats[w] = mine;
     sh.rest[w] = rest;
+    sh.rest_u[w] = rest_u;
     sh.equal[w] = equal;
   }
   __syncthreads();
   mine = lanes_join<8>(sh.stats[lane & 7]);
   rest = sh.rest[lane & 7];
+  rest_u = sh.rest_u[lane & 7];
   equal = sh.equal[lane & 7];
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) {
     rest += __shfl_xor_sync(0xffffffffu, rest, o);
+    rest_u += __shfl_xor_sync(0xffffffffu, rest_u, o);
     equal += __shfl_xor_sync(0xffffffffu, equal, o);
   }
-  if (holder < kThreads) mine.r += rest + (T)(equal - 1);
+  if (holder < kThreads) {
+    mine.r += rest + (T)(equal - 1);
+    mine.u += rest_u;
+  }
   return mine;
 }
 

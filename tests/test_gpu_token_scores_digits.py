@@ -67,3 +67,26 @@ def test_sums_over_equal_low_classes(classes, dtype):
                        (got.entropy.numpy(), np.log1p(rest) - rest * zl / (1 + rest))):
         rel = np.abs(have - want) / np.abs(want)
         assert np.all(rel <= tol), float(rel.max() / h)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64], ids=["fp32", "fp64"])
+@pytest.mark.parametrize("classes", [1000, 1500, 50304])
+def test_few_open_classes_side_by_side(classes, dtype):
+    """Open classes that one lane reads together with the maximum, all others closed."""
+    import tensorgrad_b200 as tg
+
+    rows = 96
+    low = -64 - np.arange(rows) * (977 / 4096)
+    x = np.full((rows, classes), -np.inf)
+    x[:, 400:404] = low[:, None]  # a 16-byte group in float, two of them in double
+    t = 400 + np.arange(rows) % 4
+    x[np.arange(rows), t] = 0
+    got = tg.token_log_probs(tg.Tensor(x.astype(dtype)), t)
+    zl = low.astype(np.longdouble)
+    rest = 3 * np.exp(zl)
+    h = float(np.finfo(dtype).eps) / 2
+    tol = (4 + 4 + 2 * 11 + 12) * h
+    for have, want in ((got.log_probs.numpy(), -np.log1p(rest)),
+                       (got.entropy.numpy(), np.log1p(rest) - rest * zl / (1 + rest))):
+        rel = np.abs(have - want) / np.abs(want)
+        assert np.all(rel <= tol), float(rel.max() / h)
