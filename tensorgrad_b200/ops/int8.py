@@ -100,7 +100,8 @@ def quantize_int8(x: Any) -> tuple[Tensor, Tensor]:
     """``x`` over its last axis as 8-bit integers of ``x``'s shape and one scale per row
     (``x.shape[:-1]``): ``scale = max|row| * (1 / 127)``, the factor rounded to the type, and
     the nearest integers to ``row / scale`` rounded to the type, halves to even. A row of zeros
-    has scale 0; a row with a NaN or an infinity has scale NaN and integers 0."""
+    has scale 0; a row with a NaN or an infinity has scale NaN and integers 0. Both results are
+    constants: no gradient reaches ``x`` through them, whether or not it requires one."""
     tx = as_tensor(x)
     if tx.ndim == 0 or tx.shape[-1] == 0:
         raise ValueError(f"quantize_int8 needs a last axis with values, got {tx.shape}")
