@@ -404,7 +404,9 @@ int int8_gemm_tc(const int8_t* q, const int8_t* weight, int64_t ld, const float*
   // 2304: 64 wide 8.6 us, 128 wide 9.7, 256 wide 11.5), wide ones otherwise (4096 x 768 x 50304:
   // 368, 268 and 255 us). A pair feeds 256 rows to a CTA for a 256-wide tile instead of 384, but
   // costs a round more at its start and end: it wins on long reductions of several rounds (8192 x
-  // 4096 x 4096 130 against 142 us; 2048 x 768 x 2304 13.8 against 13.2).
+  // 4096 x 4096 130 against 142 us; 2048 x 768 x 2304 13.8 against 13.2). Fewer than 96 rows a tile
+  // cost as much as 96: a round has its own latency, so 64 wide in 2 rounds beats 32 wide in 3 (16 x
+  // 4096 x 12288: 16.3 against 33.7 us, 16 x 768 x 12288: 9.2 against 10.7).
   const int64_t tm = (rows + 127) / 128, sms = tc::sm_count();
   const int64_t pairs = (rows + 255) / 256 * ((outer + 255) / 256);
   if (a.kblocks >= 16 && pairs > sms / 2)
